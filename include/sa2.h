@@ -307,6 +307,121 @@ int sa2_norm_linear(const void *x, const void *gain, int32_t gain_dtype, float e
  */
 int sa2_step_attn(const sa2_qkvnorm_args *args, const sa2_append_set sets[4], void *out, int32_t b, int32_t w1, int32_t w2, float scale);
 
+/*
+ * RMSNorm of every query and key head and the rotation by position behind it, in one pass (the reference's standard layers have
+ * neither; its sliding-window module has the norms alone, simplicial_attention/simplicial_mha.py:69-73).
+ *   u = x * rsqrt(mean over the head of x^2 + eps) * gain
+ *   the pair (u_a, u_b) turns by t = 2 pi position freqs[p] / 2^64:  y_a = u_a cos t - u_b sin t,  y_b = u_b cos t + u_a sin t
+ * Pair p < pairs is channels (p, p + pairs), or (2 p, 2 p + 1) if interleaved; channels from 2 * pairs on are normalised alone.  freqs are
+ * turns per position in units of 2^-64, so that the product with an integer position is exact modulo a turn.  positions (element
+ * strides pos_batch, pos_seq, 0 allowed) is int64; null: row i of every sequence is at start + i.
+ * x, dy: [b][n][heads][d], strides multiples of 16 bytes, 16-byte aligned; results [b][n][heads][d] contiguous.  gains: d
+ * entries, 16-byte aligned.  d is 32, 64, 128 or 256, 2 * pairs <= d and a multiple of 16, b * n below 2^31.
+ * sa2_rotary_bwd reads x again and writes dx and the gains' gradients in gain_dtype, summed in a fixed order; `partial` is scratch of
+ * sa2_rotary_partial_bytes().
+ */
+typedef struct sa2_rotary_side {
+    const void *x, *dy;        /* dy: backward only */
+    sa2_strides sx, sdy;
+    void *y;                   /* forward: y; backward: dx */
+    const void *gain;
+    void *dgain;               /* backward only */
+    int32_t heads;
+} sa2_rotary_side;
+
+typedef struct sa2_rotary_args {
+    sa2_rotary_side q, k;
+    const int64_t *freqs, *positions;
+    int64_t pos_batch, pos_seq, start;
+    void *partial;             /* backward only */
+    size_t partial_bytes;
+    int32_t b, n, d, pairs, interleaved;
+    int32_t dtype, gain_dtype;
+    float eps;
+    void *stream;
+} sa2_rotary_args;
+
+int sa2_rotary_fwd(const sa2_rotary_args *args);
+int sa2_rotary_bwd(const sa2_rotary_args *args);
+size_t sa2_rotary_partial_bytes(const sa2_rotary_args *args);
+
+/*
+ * Embedding lookup: out[r] = scale * weight[tokens[r]] + positions[start + r % n] (the reference adds two nn.Embedding modules,
+ * train.py:78-79,120-123).  All contiguous, of one dtype; tokens int64 or int32; positions may be null.  A token outside [0, vocab) reads
+ * nothing: its row of out is NaN and it has no gradient.
+ * sa2_embed_bwd writes dweight (every row) and dpositions (position_rows rows, every one); either may be null.  Sums in fp32 over sorted
+ * tokens, one order whatever the run.  The token `padding` (-1: none) has no gradient.  dweight and dpositions are 16-byte aligned, rows is
+ * below 2^31 and a multiple of n; workspace (with dweight) of sa2_embed_workspace_bytes(), 256-byte aligned.
+ */
+typedef struct sa2_embed_args {
+    const void *tokens;
+    const void *weight;        /* forward */
+    const void *positions;     /* forward */
+    void *out;                 /* forward */
+    const void *dout;          /* backward */
+    void *dweight;             /* backward */
+    void *dpositions;          /* backward */
+    void *workspace;           /* backward */
+    size_t workspace_bytes;
+    int64_t rows, vocab, start, position_rows, padding;
+    int32_t n, dim, dtype, tokens64;
+    float scale;
+    void *stream;
+} sa2_embed_args;
+
+int sa2_embed_fwd(const sa2_embed_args *args);
+int sa2_embed_bwd(const sa2_embed_args *args);
+size_t sa2_embed_workspace_bytes(int64_t rows, int32_t dim);
+
+/*
+ * Distillation from a teacher's k largest logits of a row (k <= 1024):
+ *   q = softmax(logits / T),  p = softmax(teacher / T) over the entries of the row
+ *   loss[r] = T^2 sum_k p_k (log p_k - log q[index_k]),   dlogits_j = g T (q_j - sum of p_k over index_k == j)
+ * Entries with an index outside [0, vocab) are not there; a row without entries (or with none above -inf) has loss and gradient
+ * zero.  Rows are strided, their elements contiguous; logits and dlogits fp32 or bf16 (dtype), teacher fp32 or bf16, index int64 or int32.
+ * sa2_distill_fwd writes row_loss, stats [rows][2] and counted, and total[2]: the sum of row_loss over `reduction` (SA2_SUM: 1,
+ * SA2_MEAN: the number of rows with entries, at least 1), and one over that divisor.  sa2_distill_bwd reads stats and total[1], and gout: the gradient of the
+ * total, or of every row (gout_rows != 0); null is 1.  sa2_distill_both is the forward and the backward for gout = grad_scale.
+ */
+typedef enum sa2_reduction { SA2_SUM = 0, SA2_MEAN = 1 } sa2_reduction;
+typedef struct sa2_distill_args {
+    const void *logits, *teacher, *index;
+    float *row_loss, *stats, *total;
+    int32_t *counted;
+    const float *gout;
+    void *dlogits;
+    int64_t rows, logits_stride, teacher_stride, index_stride, dlogits_stride;
+    int32_t vocab, k, dtype, teacher_dtype, index64, reduction, gout_rows;
+    float temperature, grad_scale;
+    void *stream;
+} sa2_distill_args;
+
+int sa2_distill_fwd(const sa2_distill_args *args);
+int sa2_distill_bwd(const sa2_distill_args *args);
+int sa2_distill_both(const sa2_distill_args *args);
+
+/*
+ * One token for each row of logits (fp32 or bf16, element stride 1): temperature, then the first top_k, then those before which less
+ * than top_p of the remaining mass has come, then those at least min_p times as probable as the best; of what is kept, the first token by
+ * index at which the running mass exceeds uniform[r] times the whole (the reference's sample() filters by top-k alone, train.py:104-109).
+ * Equal logits rank by index.  temperature <= 0 takes the best token; top_k <= 0 or >= vocab, top_p >= 1 and min_p <= 0 are off.  Each may be
+ * given for every row (a device pointer) or once.  A row with a NaN or +inf, or of -inf alone, gets token -1 and log-probability NaN.
+ * logprob (may be null): logarithm of the token's probability among what is kept.
+ */
+typedef struct sa2_sample_args {
+    const void *logits, *uniform;
+    const float *temperature, *top_p, *min_p;
+    const int64_t *top_k;
+    int64_t *token;
+    float *logprob;
+    int64_t rows, logits_stride, top_k_all;
+    double temperature_all, top_p_all, min_p_all;
+    int32_t vocab, dtype, uniform64;
+    void *stream;
+} sa2_sample_args;
+
+int sa2_sample(const sa2_sample_args *args);
+
 #ifdef __cplusplus
 }
 #endif

@@ -21,6 +21,7 @@
 // kernel adds the partial rows in a fixed order, without atomics.
 #pragma once
 #include "sa2_common.cuh"
+#include "sa2_vec8.cuh"
 #include <cuda_bf16.h>
 
 namespace sa2 {
@@ -29,45 +30,10 @@ namespace headnorm {
 constexpr int VEC = 8;                    // channels per lane and access
 constexpr int WARPS = 8;                  // rows per partial row at small sizes: see headnorm_grid
 
-template <typename T> __device__ __forceinline__ void load8(const T *p, float (&v)[8]);
-template <> __device__ __forceinline__ void load8<float>(const float *p, float (&v)[8]) {
-    const float4 a = *reinterpret_cast<const float4 *>(p), b = *reinterpret_cast<const float4 *>(p + 4);
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-}
-template <> __device__ __forceinline__ void load8<__nv_bfloat16>(const __nv_bfloat16 *p, float (&v)[8]) {
-    const uint4 u = *reinterpret_cast<const uint4 *>(p);
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int z = 0; z < 4; ++z) {
-        v[2 * z] = __uint_as_float(w[z] << 16);
-        v[2 * z + 1] = __uint_as_float(w[z] & 0xffff0000u);
-    }
-}
-template <typename T> __device__ __forceinline__ void store8(T *p, const float (&v)[8]);
-template <> __device__ __forceinline__ void store8<float>(float *p, const float (&v)[8]) {
-    *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]);
-    *reinterpret_cast<float4 *>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
-}
-template <> __device__ __forceinline__ void store8<__nv_bfloat16>(__nv_bfloat16 *p, const float (&v)[8]) {
-    uint32_t w[4];
-#pragma unroll
-    for (int z = 0; z < 4; ++z) {
-        const __nv_bfloat162 t = __floats2bfloat162_rn(v[2 * z], v[2 * z + 1]);
-        w[z] = *reinterpret_cast<const uint32_t *>(&t);
-    }
-    *reinterpret_cast<uint4 *>(p) = make_uint4(w[0], w[1], w[2], w[3]);
-}
-// rows whose base or stride is not a multiple of 16 bytes: element by element
-template <typename T> __device__ __forceinline__ void load8u(const T *p, bool aligned, float (&v)[8]) {
-    if (aligned) { load8<T>(p, v); return; }
-#pragma unroll
-    for (int z = 0; z < 8; ++z) v[z] = (float)p[z];
-}
-template <typename T> __device__ __forceinline__ void store8u(T *p, bool aligned, const float (&v)[8]) {
-    if (aligned) { store8<T>(p, v); return; }
-#pragma unroll
-    for (int z = 0; z < 8; ++z) p[z] = (T)v[z];
-}
+using sa2::load8;
+using sa2::load8u;
+using sa2::store8;
+using sa2::store8u;
 
 // Gain vectors.  table != null: one fp32 entry per channel.  Otherwise head h of the projection takes
 //   h < hq: p[0];   hq <= h < hq + 2 hk: p[1 + ((h - hq) & 1)];   above: p[3 + ((h - hq) & 1)]

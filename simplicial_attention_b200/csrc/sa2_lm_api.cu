@@ -1,0 +1,295 @@
+// C ABI of the operators around the attention layers (declared in include/sa2.h): argument checks and launches.  No torch types, no
+// allocation, no host sync.
+#include "sa2.h"
+#include "sa2_distill.cuh"
+#include "sa2_embed.cuh"
+#include "sa2_rotary.cuh"
+#include "sa2_sample.cuh"
+#include <nvtx3/nvToolsExt.h>
+
+namespace {
+
+constexpr int SM_COUNT = 148;     // B200
+
+struct Range {
+    explicit Range(const char *name) { nvtxRangePushA(name); }
+    ~Range() { nvtxRangePop(); }
+};
+
+inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+inline bool known(int dtype) { return dtype == SA2_F32 || dtype == SA2_BF16; }
+inline int size_of(int dtype) { return dtype == SA2_BF16 ? 2 : 4; }
+inline int launch_status() { return cudaGetLastError() == cudaSuccess ? SA2_OK : SA2_ERR_CUDA; }
+inline cudaStream_t stream_of(void *s) { return reinterpret_cast<cudaStream_t>(s); }
+
+template <typename K, typename... Args>
+int launch_clusters(K kernel, int64_t grid, int threads, size_t smem, int ctas, cudaStream_t st, const Args &...args) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return SA2_ERR_CUDA;
+    if (ctas > 8 && cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) return SA2_ERR_CUDA;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = ctas; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    cfg.gridDim = dim3((unsigned)grid); cfg.blockDim = dim3(threads); cfg.dynamicSmemBytes = smem; cfg.stream = st;
+    cfg.attrs = attr; cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess ? SA2_OK : SA2_ERR_CUDA;
+}
+
+// ---------------------------------------------------------------- queries and keys
+bool rotary_strides_ok(const sa2_strides &s, int dtype) {
+    const int piece = 16 / size_of(dtype);
+    return s.batch % piece == 0 && s.seq % piece == 0 && s.head % piece == 0;
+}
+
+int rotary_check(const sa2_rotary_args *a, bool backward) {
+    if (!a || a->b <= 0 || a->n <= 0 || a->q.heads <= 0 || a->k.heads <= 0 || !a->freqs) return SA2_ERR_INVALID;
+    if (!known(a->dtype) || !known(a->gain_dtype)) return SA2_ERR_UNSUPPORTED;
+    if (a->d != 32 && a->d != 64 && a->d != 128 && a->d != 256) return SA2_ERR_UNSUPPORTED;
+    if (a->pairs <= 0 || a->pairs % 8 || 2 * a->pairs > a->d) return SA2_ERR_UNSUPPORTED;
+    if ((int64_t)a->b * a->n > INT32_MAX || (int64_t)a->q.heads + a->k.heads > 4096) return SA2_ERR_UNSUPPORTED;
+    for (const sa2_rotary_side *s : {&a->q, &a->k}) {
+        if (!s->x || !s->y || !s->gain || !aligned16(s->x) || !aligned16(s->y) || !aligned16(s->gain) || !rotary_strides_ok(s->sx, a->dtype)) return SA2_ERR_INVALID;
+        if (backward && (!s->dy || !s->dgain || !aligned16(s->dy) || !rotary_strides_ok(s->sdy, a->dtype))) return SA2_ERR_INVALID;
+    }
+    return SA2_OK;
+}
+
+sa2::rotary::Params rotary_params(const sa2_rotary_args *a) {
+    auto side = [](const sa2_rotary_side &s) {
+        return sa2::rotary::Side{s.x, s.dy, s.sx.batch, s.sx.seq, s.sx.head, s.sdy.batch, s.sdy.seq, s.sdy.head, s.y, s.gain};
+    };
+    sa2::rotary::Params P{};
+    P.q = side(a->q); P.k = side(a->k);
+    P.freqs = a->freqs; P.positions = a->positions; P.pb = a->pos_batch; P.pn = a->pos_seq; P.start = a->start;
+    P.partial = reinterpret_cast<float *>(a->partial);
+    P.rows = (int64_t)a->b * a->n;
+    P.n = a->n; P.hq = a->q.heads; P.heads = a->q.heads + a->k.heads; P.pairs = a->pairs;
+    P.tile = sa2::rotary::tile_rows(P.rows, P.heads, a->d, a->pairs, SM_COUNT);
+    P.interleaved = a->interleaved != 0; P.gain_bf16 = a->gain_dtype == SA2_BF16; P.eps = a->eps;
+    return P;
+}
+
+template <typename T, int D> int rotary_run(const sa2::rotary::Params &P, const sa2_rotary_args *a, bool backward) {
+    using namespace sa2::rotary;
+    cudaStream_t st = stream_of(a->stream);
+    if (!backward) {
+        fwd_kernel<T, D><<<(unsigned)((P.rows + P.tile - 1) / P.tile), THREADS, fwd_smem(P.tile, P.pairs), st>>>(P);
+        return launch_status();
+    }
+    const int grid = bwd_grid(P.rows, P.tile, SM_COUNT);
+    bwd_kernel<T, D><<<grid, THREADS, bwd_smem(P.tile, P.pairs), st>>>(P);
+    if (int e = launch_status()) return e;
+    const dim3 sums(D / 32, 2);
+    if (a->gain_dtype == SA2_BF16)
+        dgain_kernel<__nv_bfloat16><<<sums, 1024, 0, st>>>(P.partial, reinterpret_cast<__nv_bfloat16 *>(a->q.dgain), reinterpret_cast<__nv_bfloat16 *>(a->k.dgain), grid, D);
+    else dgain_kernel<float><<<sums, 1024, 0, st>>>(P.partial, reinterpret_cast<float *>(a->q.dgain), reinterpret_cast<float *>(a->k.dgain), grid, D);
+    return launch_status();
+}
+
+template <typename T> int rotary_dispatch(const sa2_rotary_args *a, bool backward) {
+    const sa2::rotary::Params P = rotary_params(a);
+    switch (a->d) {
+        case 32: return rotary_run<T, 32>(P, a, backward);
+        case 64: return rotary_run<T, 64>(P, a, backward);
+        case 128: return rotary_run<T, 128>(P, a, backward);
+        default: return rotary_run<T, 256>(P, a, backward);
+    }
+}
+
+// ---------------------------------------------------------------- embedding
+int embed_check(const sa2_embed_args *a) {
+    if (!a || !a->tokens || a->rows <= 0 || a->vocab <= 0 || a->n <= 0 || a->dim <= 0) return SA2_ERR_INVALID;
+    if (!known(a->dtype) || a->rows > INT32_MAX || a->vocab > INT32_MAX) return SA2_ERR_UNSUPPORTED;
+    if (a->start < 0 || a->rows % a->n) return SA2_ERR_INVALID;
+    if ((a->positions || a->dpositions) && a->position_rows < a->start + a->n) return SA2_ERR_INVALID;
+    return SA2_OK;
+}
+
+template <typename T, int V> int embed_fwd_run(const sa2::embed::Params &P, cudaStream_t st) {
+    using namespace sa2::embed;
+    int lanes = 1;
+    while (lanes < THREADS && lanes * V < P.dim) lanes *= 2;
+    const int64_t rows = 4 * (THREADS / lanes);
+    // few rows: a CTA has a part of the channels
+    const int pieces = (P.dim + lanes * V - 1) / (lanes * V);
+    fwd_kernel<T, V><<<dim3((unsigned)((P.rows + rows - 1) / rows), (unsigned)(pieces < 64 ? pieces : 64)), THREADS, 0, st>>>(P, lanes);
+    return launch_status();
+}
+
+template <typename T> int embed_fwd(const sa2_embed_args *a) {
+    sa2::embed::Params P{a->tokens, a->tokens64, a->weight, a->positions, a->out, a->rows, a->vocab, a->start, a->n, a->dim, a->scale};
+    const bool vec = a->dim % 8 == 0 && aligned16(a->weight) && aligned16(a->out) && aligned16(a->positions);
+    return vec ? embed_fwd_run<T, 8>(P, stream_of(a->stream)) : embed_fwd_run<T, 1>(P, stream_of(a->stream));
+}
+
+template <typename T, int V> int embed_sum(const sa2::embed::BwdParams &P, cudaStream_t st) {
+    using namespace sa2::embed;
+    const int tiles = (P.dim + 32 * V - 1) / (32 * V);
+    const int64_t parts = P.dweight ? stretches(P.rows) : 0, units = (parts + (P.dpositions ? P.position_rows : 0)) * tiles;
+    if ((units + 7) / 8 > INT32_MAX || parts * tiles > INT32_MAX) return SA2_ERR_UNSUPPORTED;
+    sum_kernel<T, V><<<(unsigned)((units + 7) / 8), THREADS, 0, st>>>(P, parts, tiles);
+    if (int e = launch_status()) return e;
+    if (parts > 1) join_kernel<T, V><<<(unsigned)(parts * tiles), THREADS, 0, st>>>(P, tiles);
+    return launch_status();
+}
+
+template <typename T> int embed_bwd(const sa2_embed_args *a) {
+    using namespace sa2::embed;
+    BwdParams P{};
+    P.tokens = a->tokens; P.tokens64 = a->tokens64; P.dout = a->dout; P.dweight = a->dweight; P.dpositions = a->dpositions;
+    char *ws = reinterpret_cast<char *>(a->workspace);
+    const size_t list = up256((size_t)a->rows * 4);
+    for (int s = 0; s < 2; ++s) {
+        P.key[s] = reinterpret_cast<uint32_t *>(ws + 2 * s * list);
+        P.place[s] = reinterpret_cast<uint32_t *>(ws + (2 * s + 1) * list);
+    }
+    P.partial = reinterpret_cast<float *>(ws + 4 * list);
+    P.rows = a->rows; P.vocab = a->vocab; P.padding = a->padding; P.start = a->start; P.position_rows = a->position_rows;
+    P.n = a->n; P.dim = a->dim; P.scale = a->scale;
+    sort_plan(a->vocab, P.passes, P.bits);
+    P.vec = a->dim % 8 == 0 && aligned16(a->dout) && aligned16(a->dweight) && aligned16(a->dpositions);
+    cudaStream_t st = stream_of(a->stream);
+    if (!P.dweight) return P.vec ? embed_sum<T, 8>(P, st) : embed_sum<T, 1>(P, st);
+    // one cluster sorts; the others have 64 KB of zeros each to write, up to two CTAs an SM
+    const int ctas = sort_ctas(a->rows);
+    const int64_t bytes = a->vocab * a->dim * (int64_t)sizeof(T);
+    int64_t fill = (bytes + 65535) / 65536;
+    if (fill > 2 * SM_COUNT) fill = 2 * SM_COUNT;
+    fill = (fill + ctas - 1) / ctas * ctas;
+    if (int e = launch_clusters(sort_kernel, ctas + fill, SORT_THREADS, sort_smem(P.bits), ctas, st, P, bytes)) return e;
+    return P.vec ? embed_sum<T, 8>(P, st) : embed_sum<T, 1>(P, st);
+}
+
+// ---------------------------------------------------------------- distillation
+int distill_check(const sa2_distill_args *a, bool forward, bool backward) {
+    if (!a || !a->logits || !a->teacher || !a->index || !a->stats || !a->total || a->rows <= 0 || a->vocab <= 0 || a->k <= 0) return SA2_ERR_INVALID;
+    if (forward && (!a->row_loss || !a->counted)) return SA2_ERR_INVALID;
+    if (backward && !a->dlogits) return SA2_ERR_INVALID;
+    if (!known(a->dtype) || !known(a->teacher_dtype) || a->k > sa2::distill::MAX_K || a->rows > INT32_MAX) return SA2_ERR_UNSUPPORTED;
+    if (a->reduction != SA2_SUM && a->reduction != SA2_MEAN) return SA2_ERR_UNSUPPORTED;
+    if (!(a->temperature > 0.f) || a->temperature * 0.f != 0.f) return SA2_ERR_INVALID;
+    const uintptr_t unit = size_of(a->dtype) - 1;
+    if ((reinterpret_cast<uintptr_t>(a->logits) & unit) || (backward && (reinterpret_cast<uintptr_t>(a->dlogits) & unit))) return SA2_ERR_INVALID;
+    return SA2_OK;
+}
+
+sa2::distill::Params distill_params(const sa2_distill_args *a) {
+    sa2::distill::Params P{};
+    P.z = a->logits; P.teacher = a->teacher; P.index = a->index; P.stats = a->stats; P.row_loss = a->row_loss; P.counted = a->counted;
+    P.dz = a->dlogits; P.gout = a->gout; P.gs = a->gout_rows != 0;
+    P.scale = a->reduction == SA2_MEAN && !a->gout_rows ? a->total + 1 : nullptr;
+    P.times = a->grad_scale;
+    P.rows = a->rows; P.zs = a->logits_stride; P.ts = a->teacher_stride; P.is = a->index_stride; P.ds = a->dlogits_stride;
+    P.vocab = a->vocab; P.k = a->k; P.index64 = a->index64; P.teacher_bf16 = a->teacher_dtype == SA2_BF16; P.t = a->temperature;
+    return P;
+}
+
+// a warp a row up to this vocabulary
+constexpr int WARP_VOCAB = 2048;
+
+template <typename T> int distill_fwd(const sa2_distill_args *a) {
+    const sa2::distill::Params P = distill_params(a);
+    cudaStream_t st = stream_of(a->stream);
+    if (a->vocab <= WARP_VOCAB) sa2::distill::fwd_kernel<T, 32><<<(unsigned)((a->rows + 7) / 8), 256, 0, st>>>(P);
+    else sa2::distill::fwd_kernel<T, 512><<<(unsigned)a->rows, 512, 0, st>>>(P);
+    if (int e = launch_status()) return e;
+    sa2::distill::total_kernel<<<1, 1024, 0, st>>>(a->row_loss, a->counted, a->rows, a->reduction == SA2_MEAN, a->total);
+    return launch_status();
+}
+
+template <typename T> int distill_bwd(const sa2_distill_args *a) {
+    const sa2::distill::Params P = distill_params(a);
+    cudaStream_t st = stream_of(a->stream);
+    const size_t entries = (size_t)a->k * 8;
+    if (a->vocab <= WARP_VOCAB) {
+        const auto kernel = sa2::distill::bwd_kernel<T, 32>;
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 8 * sa2::distill::MAX_K * 8) != cudaSuccess) return SA2_ERR_CUDA;
+        kernel<<<(unsigned)((a->rows + 7) / 8), 256, 8 * entries, st>>>(P);
+    } else {
+        sa2::distill::bwd_kernel<T, 512><<<(unsigned)a->rows, 512, entries, st>>>(P);
+    }
+    return launch_status();
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t sa2_rotary_partial_bytes(const sa2_rotary_args *a) {
+    if (!a || a->b <= 0 || a->n <= 0 || a->q.heads <= 0 || a->k.heads <= 0 || a->d <= 0 || a->pairs <= 0) return 0;
+    const int64_t rows = (int64_t)a->b * a->n;
+    const int tile = sa2::rotary::tile_rows(rows, a->q.heads + a->k.heads, a->d, a->pairs, SM_COUNT);
+    return (size_t)sa2::rotary::bwd_grid(rows, tile, SM_COUNT) * 2 * a->d * sizeof(float);
+}
+int sa2_rotary_fwd(const sa2_rotary_args *a) {
+    Range range("sa2_rotary_fwd");
+    if (int e = rotary_check(a, false)) return e;
+    return a->dtype == SA2_BF16 ? rotary_dispatch<__nv_bfloat16>(a, false) : rotary_dispatch<float>(a, false);
+}
+int sa2_rotary_bwd(const sa2_rotary_args *a) {
+    Range range("sa2_rotary_bwd");
+    if (int e = rotary_check(a, true)) return e;
+    if (!a->partial || !aligned16(a->partial) || a->partial_bytes < sa2_rotary_partial_bytes(a)) return SA2_ERR_WORKSPACE;
+    return a->dtype == SA2_BF16 ? rotary_dispatch<__nv_bfloat16>(a, true) : rotary_dispatch<float>(a, true);
+}
+
+size_t sa2_embed_workspace_bytes(int64_t rows, int32_t dim) {
+    return rows > 0 && dim > 0 ? sa2::embed::workspace_bytes(rows, dim) : 0;
+}
+int sa2_embed_fwd(const sa2_embed_args *a) {
+    Range range("sa2_embed_fwd");
+    if (int e = embed_check(a)) return e;
+    if (!a->weight || !a->out) return SA2_ERR_INVALID;
+    return a->dtype == SA2_BF16 ? embed_fwd<__nv_bfloat16>(a) : embed_fwd<float>(a);
+}
+int sa2_embed_bwd(const sa2_embed_args *a) {
+    Range range("sa2_embed_bwd");
+    if (int e = embed_check(a)) return e;
+    if (!a->dout || (!a->dweight && !a->dpositions) || !aligned16(a->dweight) || !aligned16(a->dpositions)) return SA2_ERR_INVALID;
+    if (a->dweight && (!a->workspace || (reinterpret_cast<uintptr_t>(a->workspace) & 255u) || a->workspace_bytes < sa2_embed_workspace_bytes(a->rows, a->dim)))
+        return SA2_ERR_WORKSPACE;
+    return a->dtype == SA2_BF16 ? embed_bwd<__nv_bfloat16>(a) : embed_bwd<float>(a);
+}
+
+int sa2_distill_fwd(const sa2_distill_args *a) {
+    Range range("sa2_distill_fwd");
+    if (int e = distill_check(a, true, false)) return e;
+    return a->dtype == SA2_BF16 ? distill_fwd<__nv_bfloat16>(a) : distill_fwd<float>(a);
+}
+int sa2_distill_bwd(const sa2_distill_args *a) {
+    Range range("sa2_distill_bwd");
+    if (int e = distill_check(a, false, true)) return e;
+    return a->dtype == SA2_BF16 ? distill_bwd<__nv_bfloat16>(a) : distill_bwd<float>(a);
+}
+int sa2_distill_both(const sa2_distill_args *a) {
+    Range range("sa2_distill_both");
+    if (int e = distill_check(a, true, true)) return e;
+    if (a->gout) return SA2_ERR_INVALID;
+    if (int e = a->dtype == SA2_BF16 ? distill_fwd<__nv_bfloat16>(a) : distill_fwd<float>(a)) return e;
+    return a->dtype == SA2_BF16 ? distill_bwd<__nv_bfloat16>(a) : distill_bwd<float>(a);
+}
+
+int sa2_sample(const sa2_sample_args *a) {
+    Range range("sa2_sample");
+    if (!a || !a->logits || !a->uniform || !a->token || a->rows <= 0 || a->vocab <= 0) return SA2_ERR_INVALID;
+    if (!known(a->dtype)) return SA2_ERR_UNSUPPORTED;
+    if (reinterpret_cast<uintptr_t>(a->logits) & (size_of(a->dtype) - 1)) return SA2_ERR_INVALID;
+    namespace sm = sa2::sample;
+    sm::Params P{};
+    P.z = a->logits; P.uniform = a->uniform; P.temperature = a->temperature; P.top_p = a->top_p; P.min_p = a->min_p; P.top_k = a->top_k;
+    P.token = a->token; P.logprob = a->logprob; P.rows = a->rows; P.zs = a->logits_stride;
+    P.top_k_all = a->top_k_all; P.temperature_all = a->temperature_all; P.top_p_all = a->top_p_all; P.min_p_all = a->min_p_all;
+    P.vocab = a->vocab; P.uniform64 = a->uniform64;
+    const int size = size_of(a->dtype), ctas = sm::ctas_of(a->rows, a->vocab, size, SM_COUNT);
+    P.slice = sm::slice_of(a->vocab, ctas);
+    P.shift = sm::mass_shift(a->vocab);
+    size_t smem = sizeof(sm::Shared) + (size_t)P.slice * size;
+    P.resident = smem <= 200 * 1024;
+    if (!P.resident) smem = sizeof(sm::Shared);
+    if (a->rows * ctas > INT32_MAX) return SA2_ERR_UNSUPPORTED;
+    cudaStream_t st = stream_of(a->stream);
+    return a->dtype == SA2_BF16 ? launch_clusters(sm::kernel<__nv_bfloat16>, a->rows * ctas, sm::THREADS, smem, ctas, st, P)
+                                : launch_clusters(sm::kernel<float>, a->rows * ctas, sm::THREADS, smem, ctas, st, P);
+}
+
+}  // extern "C"

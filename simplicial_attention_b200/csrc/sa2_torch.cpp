@@ -35,6 +35,16 @@ struct Lib {
     int (*append)(const sa2_qkvnorm_args *, const sa2_append_set *, int32_t, int32_t) = nullptr;
     int (*norm_linear)(const void *, const void *, int32_t, float, const void *, void *, int32_t, int32_t, int32_t, void *) = nullptr;
     int (*step_attn)(const sa2_qkvnorm_args *, const sa2_append_set *, void *, int32_t, int32_t, int32_t, float) = nullptr;
+    int (*rotary_fwd)(const sa2_rotary_args *) = nullptr;
+    int (*rotary_bwd)(const sa2_rotary_args *) = nullptr;
+    size_t (*rotary_partial)(const sa2_rotary_args *) = nullptr;
+    int (*embed_fwd)(const sa2_embed_args *) = nullptr;
+    int (*embed_bwd)(const sa2_embed_args *) = nullptr;
+    size_t (*embed_workspace)(int64_t, int32_t) = nullptr;
+    int (*distill_fwd)(const sa2_distill_args *) = nullptr;
+    int (*distill_bwd)(const sa2_distill_args *) = nullptr;
+    int (*distill_both)(const sa2_distill_args *) = nullptr;
+    int (*sample)(const sa2_sample_args *) = nullptr;
 } L;
 
 void bind(const std::map<std::string, uintptr_t> &f) {
@@ -43,6 +53,10 @@ void bind(const std::map<std::string, uintptr_t> &f) {
     set(L.norm_fwd, "sa2_headnorm_fwd"); set(L.norm_bwd, "sa2_headnorm_bwd"); set(L.partial_bytes, "sa2_headnorm_partial_bytes");
     set(L.qkv_fwd, "sa2_qkvnorm_fwd"); set(L.qkv_bwd, "sa2_qkvnorm_bwd"); set(L.append, "sa2_qkv_append");
     set(L.norm_linear, "sa2_norm_linear"); set(L.step_attn, "sa2_step_attn");
+    set(L.rotary_fwd, "sa2_rotary_fwd"); set(L.rotary_bwd, "sa2_rotary_bwd"); set(L.rotary_partial, "sa2_rotary_partial_bytes");
+    set(L.embed_fwd, "sa2_embed_fwd"); set(L.embed_bwd, "sa2_embed_bwd"); set(L.embed_workspace, "sa2_embed_workspace_bytes");
+    set(L.distill_fwd, "sa2_distill_fwd"); set(L.distill_bwd, "sa2_distill_bwd"); set(L.distill_both, "sa2_distill_both");
+    set(L.sample, "sa2_sample");
 }
 
 // raises _lib.Sa2Error, also from the autograd engine's threads
@@ -468,9 +482,304 @@ pybind11::object step(const Tensor &x, const std::optional<Tensor> &pre, double 
     return pybind11::make_tuple(out, set[0], set[1], set[2], set[3]);
 }
 
+// ------------------------------------------------------------------ what is around the attention layers
+void *stream_of(const Tensor &t) { return c10::cuda::getCurrentCUDAStream(t.get_device()).stream(); }
+// create_graph: the nodes below have no second derivative
+void once(const char *what) {
+    TORCH_CHECK(!at::GradMode::is_enabled(), what, ": the backward has no backward of its own (create_graph=True)");
+}
+
+// queries or keys [b][n][h][d] as the kernel reads them (the stride of a dimension of one element is any), or a copy
+sa2_strides head_strides(const Tensor &t) {
+    auto st = [&](int x) { return t.size(x) == 1 ? (int64_t)0 : t.stride(x); };
+    return sa2_strides{st(0), st(1), st(2)};
+}
+Tensor head_rows(const Tensor &t) {
+    const int64_t piece = t.scalar_type() == at::kBFloat16 ? 8 : 4;
+    const sa2_strides s = head_strides(t);
+    return t.stride(3) == 1 && s.batch % piece == 0 && s.seq % piece == 0 && s.head % piece == 0 && aligned(t) ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+Tensor packed(const Tensor &t) { return t.is_contiguous() && aligned(t) ? t : t.clone(at::MemoryFormat::Contiguous); }
+
+struct Rotary : torch::autograd::Function<Rotary> {
+    static void fill(sa2_rotary_args &a, const Tensor &q, const Tensor &k, const Tensor &gq, const Tensor &gk, const Tensor &freqs, const Tensor &positions,
+                     int64_t start, double eps, bool interleaved) {
+        a.q.x = q.data_ptr(); a.q.sx = head_strides(q); a.q.gain = gq.data_ptr(); a.q.heads = (int32_t)q.size(2);
+        a.k.x = k.data_ptr(); a.k.sx = head_strides(k); a.k.gain = gk.data_ptr(); a.k.heads = (int32_t)k.size(2);
+        a.freqs = freqs.data_ptr<int64_t>();
+        if (positions.defined()) {
+            a.positions = positions.data_ptr<int64_t>();
+            a.pos_seq = positions.stride(-1);
+            a.pos_batch = positions.dim() == 2 && positions.size(0) > 1 ? positions.stride(0) : 0;
+        }
+        a.start = start;
+        a.b = (int32_t)q.size(0); a.n = (int32_t)q.size(1); a.d = (int32_t)q.size(3); a.pairs = (int32_t)freqs.size(0); a.interleaved = interleaved;
+        a.dtype = dtype_of(q); a.gain_dtype = dtype_of(gq); a.eps = (float)eps; a.stream = stream_of(q);
+    }
+    static variable_list forward(AutogradContext *ctx, const Tensor &q, const Tensor &k, const Tensor &gq, const Tensor &gk, const Tensor &freqs,
+                                 const std::optional<Tensor> &places, int64_t start, double eps, bool interleaved) {
+        const c10::cuda::CUDAGuard guard(q.device());
+        const Tensor positions = places.value_or(Tensor());
+        Tensor yq = at::empty(q.sizes(), q.options()), yk = at::empty(k.sizes(), k.options());
+        if (q.size(0) && q.size(1)) {
+            const Tensor x = head_rows(q), y = head_rows(k), g = packed(gq), h = packed(gk), f = freqs.contiguous();
+            sa2_rotary_args a{};
+            fill(a, x, y, g, h, f, positions, start, eps, interleaved);
+            a.q.y = yq.data_ptr(); a.k.y = yk.data_ptr();
+            check(L.rotary_fwd(&a), "sa2_rotary_fwd");
+        }
+        ctx->save_for_backward({q, k, gq, gk, freqs, positions});
+        ctx->saved_data["start"] = start;
+        ctx->saved_data["eps"] = eps;
+        ctx->saved_data["interleaved"] = interleaved;
+        return {yq, yk};
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grads) {
+        once("qk_norm_rotary");
+        const auto s = ctx->get_saved_variables();
+        const c10::cuda::CUDAGuard guard(s[0].device());
+        Tensor g[4];
+        for (int x = 0; x < 4; ++x) g[x] = at::empty(s[x].sizes(), s[x].options().memory_format(at::MemoryFormat::Contiguous));
+        if (s[0].size(0) && s[0].size(1)) {
+            const Tensor q = head_rows(s[0]), k = head_rows(s[1]), gq = packed(s[2]), gk = packed(s[3]), f = s[4].contiguous();
+            const Tensor dq = head_rows(grads[0].to(q.scalar_type())), dk = head_rows(grads[1].to(q.scalar_type()));
+            sa2_rotary_args a{};
+            fill(a, q, k, gq, gk, f, s[5], ctx->saved_data["start"].toInt(), ctx->saved_data["eps"].toDouble(), ctx->saved_data["interleaved"].toBool());
+            a.q.dy = dq.data_ptr(); a.q.sdy = head_strides(dq); a.q.y = g[0].data_ptr(); a.q.dgain = g[2].data_ptr();
+            a.k.dy = dk.data_ptr(); a.k.sdy = head_strides(dk); a.k.y = g[1].data_ptr(); a.k.dgain = g[3].data_ptr();
+            const Tensor partial = at::empty({(int64_t)L.rotary_partial(&a)}, q.options().dtype(at::kByte));
+            a.partial = partial.data_ptr(); a.partial_bytes = (size_t)partial.numel();
+            check(L.rotary_bwd(&a), "sa2_rotary_bwd");
+        } else {
+            g[2].zero_();
+            g[3].zero_();
+        }
+        return {g[0], g[1], g[2], g[3], Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+    }
+};
+
+// (queries, keys), or None
+pybind11::object qk_norm_rotary(const Tensor &q, const Tensor &k, const Tensor &gq, const Tensor &gk, const Tensor &freqs, const std::optional<Tensor> &positions,
+                                int64_t start, double eps, bool interleaved) {
+    if (tracing()) return pybind11::none();
+    for (const Tensor *t : {&q, &k, &gq, &gk, &freqs})
+        if (!plain(*t, q.device())) return pybind11::none();
+    if (positions && !plain(*positions, q.device())) return pybind11::none();
+    if (q.dim() != 4 || k.dim() != 4 || dtype_of(q) < 0 || k.scalar_type() != q.scalar_type() || q.size(0) != k.size(0) || q.size(1) != k.size(1) || q.size(3) != k.size(3) ||
+        q.size(2) == 0 || k.size(2) == 0 || q.size(2) + k.size(2) > 4096) return pybind11::none();
+    const int64_t d = q.size(3);
+    if (d != 32 && d != 64 && d != 128 && d != 256) return pybind11::none();
+    for (const Tensor *t : {&gq, &gk})
+        if (t->dim() != 1 || t->size(0) != d || dtype_of(*t) < 0 || t->scalar_type() != gq.scalar_type()) return pybind11::none();
+    if (freqs.dim() != 1 || freqs.scalar_type() != at::kLong || freqs.size(0) == 0 || freqs.size(0) % 8 || 2 * freqs.size(0) > d) return pybind11::none();
+    if (positions) {
+        const Tensor &p = *positions;
+        const bool whole = p.dim() == 2 && (p.size(0) == q.size(0) || p.size(0) == 1);
+        if (p.scalar_type() != at::kLong || !(p.dim() == 1 || whole) || p.size(-1) != q.size(1)) return pybind11::none();
+    }
+    if (q.size(0) * q.size(1) > INT32_MAX) return pybind11::none();
+    const auto r = Rotary::apply(q, k, gq, gk, freqs, positions, start, eps, interleaved);
+    return pybind11::make_tuple(r[0], r[1]);
+}
+
+struct Embed : torch::autograd::Function<Embed> {
+    static void fill(sa2_embed_args &a, const Tensor &tokens, const Tensor &like, int64_t n, int64_t vocab, int64_t start, int64_t position_rows,
+                     int64_t padding, double scale) {
+        a.tokens = tokens.data_ptr(); a.tokens64 = tokens.scalar_type() == at::kLong;
+        a.rows = tokens.numel(); a.vocab = vocab; a.start = start; a.position_rows = position_rows; a.padding = padding;
+        a.n = (int32_t)n; a.dim = (int32_t)like.size(-1); a.dtype = dtype_of(like); a.scale = (float)scale; a.stream = stream_of(like);
+    }
+    static Tensor forward(AutogradContext *ctx, const Tensor &tokens, const Tensor &weight, const std::optional<Tensor> &table, double scale, int64_t start, int64_t padding) {
+        const c10::cuda::CUDAGuard guard(weight.device());
+        const Tensor positions = table.value_or(Tensor());
+        auto shape = tokens.sizes().vec();
+        const int64_t n = shape.empty() ? 1 : shape.back();
+        shape.push_back(weight.size(1));
+        Tensor out = at::empty(shape, weight.options());
+        const Tensor t = tokens.contiguous();
+        if (t.numel()) {
+            const Tensor w = weight.contiguous(), p = positions.defined() ? positions.contiguous() : positions;
+            sa2_embed_args a{};
+            fill(a, t, w, n, weight.size(0), start, p.defined() ? p.size(0) : 0, padding, scale);
+            a.weight = w.data_ptr(); a.positions = p.defined() ? p.data_ptr() : nullptr; a.out = out.data_ptr();
+            check(L.embed_fwd(&a), "sa2_embed_fwd");
+        }
+        ctx->save_for_backward({t});
+        ctx->saved_data["i"] = std::vector<int64_t>{n, weight.size(0), start, positions.defined() ? positions.size(0) : -1, padding};
+        ctx->saved_data["scale"] = scale;
+        return out;
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grads) {
+        const Tensor tokens = ctx->get_saved_variables()[0];
+        const c10::cuda::CUDAGuard guard(tokens.device());
+        const auto i = ctx->saved_data["i"].toIntVector();
+        const int64_t n = i[0], vocab = i[1], start = i[2], position_rows = i[3], padding = i[4], dim = grads[0].size(-1);
+        const double scale = ctx->saved_data["scale"].toDouble();
+        const bool want_w = ctx->needs_input_grad(1), want_p = position_rows >= 0 && ctx->needs_input_grad(2);
+        Tensor dw, dp;
+        if (at::GradMode::is_enabled()) {                // a backward of this backward: in torch's operators
+            if (want_w) dw = at::embedding_dense_backward(grads[0] * scale, tokens.to(at::kLong), vocab, padding, false);
+            if (want_p) dp = at::constant_pad_nd(grads[0].reshape({-1, n, dim}).sum(0), {0, 0, start, position_rows - start - n});
+        } else {
+            const Tensor dout = grads[0].contiguous();
+            if (want_w) dw = at::empty({vocab, dim}, dout.options());
+            if (want_p) dp = at::empty({position_rows, dim}, dout.options());
+            if (tokens.numel() && (want_w || want_p)) {
+                const Tensor ws = at::empty({want_w ? (int64_t)L.embed_workspace(tokens.numel(), (int32_t)dim) : 256}, dout.options().dtype(at::kByte));
+                sa2_embed_args a{};
+                fill(a, tokens, dout, n, vocab, start, want_p ? position_rows : 0, padding, scale);
+                a.dout = dout.data_ptr(); a.dweight = want_w ? dw.data_ptr() : nullptr; a.dpositions = want_p ? dp.data_ptr() : nullptr;
+                a.workspace = ws.data_ptr(); a.workspace_bytes = (size_t)ws.numel();
+                check(L.embed_bwd(&a), "sa2_embed_bwd");
+            } else {
+                if (want_w) dw.zero_();
+                if (want_p) dp.zero_();
+            }
+        }
+        return {Tensor(), dw, dp, Tensor(), Tensor(), Tensor()};
+    }
+};
+
+// [...][dim], or None
+pybind11::object embed(const Tensor &tokens, const Tensor &weight, const std::optional<Tensor> &positions, double scale, int64_t start, int64_t padding) {
+    if (tracing() || !plain(weight, weight.device()) || !plain(tokens, weight.device()) || (positions && !plain(*positions, weight.device()))) return pybind11::none();
+    if ((tokens.scalar_type() != at::kLong && tokens.scalar_type() != at::kInt) || weight.dim() != 2 || dtype_of(weight) < 0 || weight.numel() == 0) return pybind11::none();
+    if (tokens.numel() > INT32_MAX || weight.size(0) > INT32_MAX || weight.size(1) > INT32_MAX) return pybind11::none();
+    const int64_t n = tokens.dim() ? tokens.size(-1) : 1;
+    if (positions && (positions->dim() != 2 || positions->size(1) != weight.size(1) || positions->scalar_type() != weight.scalar_type() || start < 0 || start + n > positions->size(0)))
+        return pybind11::none();
+    return pybind11::cast(Embed::apply(tokens, weight, positions, scale, start, padding));
+}
+
+// reduction: SA2_SUM, SA2_MEAN, or 2 for none
+constexpr int64_t NONE = 2;
+struct Distill : torch::autograd::Function<Distill> {
+    static void fill(sa2_distill_args &a, const Tensor &logits, const Tensor &teacher, const Tensor &index, const Tensor &stats, const Tensor &total, double t, int64_t reduction) {
+        a.logits = logits.data_ptr(); a.teacher = teacher.data_ptr(); a.index = index.data_ptr();
+        a.stats = stats.data_ptr<float>(); a.total = total.data_ptr<float>();
+        a.rows = logits.size(0); a.logits_stride = logits.stride(0); a.teacher_stride = teacher.stride(0); a.index_stride = index.stride(0);
+        a.vocab = (int32_t)logits.size(1); a.k = (int32_t)teacher.size(1);
+        a.dtype = dtype_of(logits); a.teacher_dtype = dtype_of(teacher); a.index64 = index.scalar_type() == at::kLong;
+        a.reduction = reduction == SA2_MEAN ? SA2_MEAN : SA2_SUM; a.temperature = (float)t; a.grad_scale = 1.f; a.stream = stream_of(logits);
+    }
+    static Tensor flat(const Tensor &t) {
+        const Tensor r = t.dim() == 2 ? t : t.reshape({-1, t.size(-1)});
+        return r.stride(1) == 1 || r.size(1) == 1 ? r : r.contiguous();
+    }
+    // loss and the statistics of the rows; with `grad` also the gradient times `grad_scale`
+    static Tensor run(const Tensor &z, const Tensor &teacher, const Tensor &index, double t, int64_t reduction, Tensor &stats, Tensor &total, const Tensor &grad, double grad_scale) {
+        const auto f32 = z.options().dtype(at::kFloat);
+        const int64_t rows = z.size(0);
+        stats = at::empty({rows, 2}, f32);
+        total = at::empty({2}, f32);
+        const Tensor losses = at::empty({rows}, f32), counted = at::empty({rows}, z.options().dtype(at::kInt));
+        if (rows == 0) {
+            total.zero_();
+        } else {
+            sa2_distill_args a{};
+            fill(a, z, teacher, index, stats, total, t, reduction);
+            a.row_loss = losses.data_ptr<float>(); a.counted = counted.data_ptr<int32_t>(); a.grad_scale = (float)grad_scale;
+            if (grad.defined()) {
+                a.dlogits = grad.data_ptr(); a.dlogits_stride = grad.stride(0);
+                check(L.distill_both(&a), "sa2_distill_both");
+            } else {
+                check(L.distill_fwd(&a), "sa2_distill_fwd");
+            }
+        }
+        return reduction == NONE ? losses : total.select(0, 0);
+    }
+    static Tensor forward(AutogradContext *ctx, const Tensor &logits, const Tensor &teacher, const Tensor &index, double t, int64_t reduction) {
+        const c10::cuda::CUDAGuard guard(logits.device());
+        const Tensor z = flat(logits), te = flat(teacher), ix = flat(index);
+        Tensor stats, total;
+        Tensor loss = run(z, te, ix, t, reduction, stats, total, Tensor(), 1.);
+        // (a tensor of its own: the caller may write into the loss)
+        loss = reduction == NONE ? loss.view(logits.sizes().slice(0, logits.dim() - 1)) : loss.clone();
+        ctx->save_for_backward({z, te, ix, stats, total});
+        ctx->saved_data["t"] = t;
+        ctx->saved_data["reduction"] = reduction;
+        ctx->saved_data["shape"] = logits.sizes().vec();
+        return loss;
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grads) {
+        once("distillation_loss");
+        const auto s = ctx->get_saved_variables();
+        const Tensor &z = s[0];
+        const c10::cuda::CUDAGuard guard(z.device());
+        const int64_t reduction = ctx->saved_data["reduction"].toInt();
+        Tensor grad = at::empty(z.sizes(), z.options().memory_format(at::MemoryFormat::Contiguous));
+        if (grad.numel()) {
+            const Tensor gout = grads[0].reshape({-1}).to(at::kFloat).contiguous();
+            sa2_distill_args a{};
+            fill(a, z, s[1], s[2], s[3], s[4], ctx->saved_data["t"].toDouble(), reduction);
+            a.gout = gout.data_ptr<float>(); a.gout_rows = reduction == NONE;
+            a.dlogits = grad.data_ptr(); a.dlogits_stride = grad.stride(0);
+            check(L.distill_bwd(&a), "sa2_distill_bwd");
+        }
+        return {grad.view(ctx->saved_data["shape"].toIntVector()), Tensor(), Tensor(), Tensor(), Tensor()};
+    }
+};
+
+bool distill_ok(const Tensor &logits, const Tensor &teacher, const Tensor &index) {
+    if (tracing()) return false;
+    for (const Tensor *t : {&logits, &teacher, &index})
+        if (!plain(*t, logits.device()) || t->dim() < 1 || t->dim() != logits.dim() || t->sizes().slice(0, t->dim() - 1) != logits.sizes().slice(0, logits.dim() - 1)) return false;
+    if (dtype_of(logits) < 0 || dtype_of(teacher) < 0 || (index.scalar_type() != at::kLong && index.scalar_type() != at::kInt)) return false;
+    const int64_t vocab = logits.size(-1), k = teacher.size(-1);
+    return vocab > 0 && vocab <= INT32_MAX && k > 0 && k <= 1024 && index.size(-1) == k && logits.numel() / vocab <= INT32_MAX;
+}
+pybind11::object distill(const Tensor &logits, const Tensor &teacher, const Tensor &index, double t, int64_t reduction) {
+    if (!distill_ok(logits, teacher, index)) return pybind11::none();
+    return pybind11::cast(Distill::apply(logits, teacher, index, t, reduction));
+}
+// (loss, gradient), or None
+pybind11::object distill_both(const Tensor &logits, const Tensor &teacher, const Tensor &index, double t, int64_t reduction, double grad_scale) {
+    if (!distill_ok(logits, teacher, index)) return pybind11::none();
+    const c10::cuda::CUDAGuard guard(logits.device());
+    const at::AutoDispatchBelowADInplaceOrView below;
+    const Tensor z = Distill::flat(logits);
+    Tensor grad = at::empty(z.sizes(), z.options().memory_format(at::MemoryFormat::Contiguous)), stats, total;
+    const Tensor loss = Distill::run(z, Distill::flat(teacher), Distill::flat(index), t, reduction, stats, total, grad, grad_scale);
+    return pybind11::make_tuple(loss, grad.view(logits.sizes()));
+}
+
+// (tokens, log-probabilities or None), or None.  The tensors of settings are [rows], contiguous.
+pybind11::object sample(const Tensor &logits, const Tensor &uniform, const std::optional<Tensor> &temperature, double temperature_all, const std::optional<Tensor> &top_k,
+                        int64_t top_k_all, const std::optional<Tensor> &top_p, double top_p_all, const std::optional<Tensor> &min_p, double min_p_all, bool logprobs) {
+    if (tracing() || !plain(logits, logits.device()) || !plain(uniform, logits.device()) || logits.dim() < 1 || dtype_of(logits) < 0) return pybind11::none();
+    const auto shape = logits.sizes().slice(0, logits.dim() - 1);
+    if (uniform.sizes() != shape || (uniform.scalar_type() != at::kFloat && uniform.scalar_type() != at::kDouble) || logits.size(-1) == 0 || logits.size(-1) > INT32_MAX) return pybind11::none();
+    const int64_t vocab = logits.size(-1), rows = logits.numel() / vocab;
+    for (const auto *t : {&temperature, &top_p, &min_p})
+        if (*t && (!plain(**t, logits.device()) || (*t)->scalar_type() != at::kFloat || (*t)->numel() != rows || !(*t)->is_contiguous())) return pybind11::none();
+    if (top_k && (!plain(*top_k, logits.device()) || top_k->scalar_type() != at::kLong || top_k->numel() != rows || !top_k->is_contiguous())) return pybind11::none();
+    const c10::cuda::CUDAGuard guard(logits.device());
+    const at::AutoDispatchBelowADInplaceOrView below;
+    Tensor token = at::empty(shape, logits.options().dtype(at::kLong)), logprob;
+    if (logprobs) logprob = at::empty(shape, logits.options().dtype(at::kFloat));
+    if (rows) {
+        const Tensor z = Distill::flat(logits), u = uniform.contiguous();
+        sa2_sample_args a{};
+        a.logits = z.data_ptr(); a.uniform = u.data_ptr(); a.uniform64 = u.scalar_type() == at::kDouble;
+        a.temperature = temperature ? temperature->data_ptr<float>() : nullptr; a.temperature_all = temperature_all;
+        a.top_k = top_k ? top_k->data_ptr<int64_t>() : nullptr; a.top_k_all = top_k_all;
+        a.top_p = top_p ? top_p->data_ptr<float>() : nullptr; a.top_p_all = top_p_all;
+        a.min_p = min_p ? min_p->data_ptr<float>() : nullptr; a.min_p_all = min_p_all;
+        a.token = token.data_ptr<int64_t>(); a.logprob = logprobs ? logprob.data_ptr<float>() : nullptr;
+        a.rows = rows; a.logits_stride = z.stride(0); a.vocab = (int32_t)vocab; a.dtype = dtype_of(z); a.stream = stream_of(z);
+        check(L.sample(&a), "sa2_sample");
+    }
+    return pybind11::make_tuple(token, logprobs ? pybind11::cast(logprob) : pybind11::none());
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+    m.def("qk_norm_rotary", &qk_norm_rotary);
+    m.def("embed", &embed);
+    m.def("distill", &distill);
+    m.def("distill_both", &distill_both);
+    m.def("sample", &sample);
     m.def("bind", &bind);
     m.def("attn", &attn);
     m.def("headnorm", &headnorm);

@@ -1,0 +1,224 @@
+"""Distillation from a teacher's top logits against 64 bits.
+
+Tolerances, with u = 2^-24: a weight 2^x is off by 4 u (ex2) and by 2 u |x| (its exponent's roundings), the sum of a row by at most
+(vocab / 32 + 64) u more, the logarithm and the probabilities by the same.  `slack` below is the sum of these; results are rounded to
+their types."""
+import pytest
+import torch
+
+import simplicial_attention_b200 as sa
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+
+
+def _half_step(t):
+    return torch.finfo(t.dtype).eps / 2
+
+
+def _inputs(rows, vocab, k, dtype, teacher_dtype=torch.float32, seed=0, spread=3.0):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    z = (torch.randn(rows, vocab, generator=gen, device="cuda") * spread).to(dtype)
+    t = (torch.randn(rows, k, generator=gen, device="cuda") * spread).to(teacher_dtype)
+    i = torch.rand(rows, vocab, generator=gen, device="cuda").argsort(-1)[:, :k]
+    if k > vocab:
+        i = torch.randint(vocab, (rows, k), generator=gen, device="cuda")
+    return z, t, i.contiguous()
+
+
+def _oracle(z, t, i, temperature):
+    """Loss of every row, its gradient, whether the row counts."""
+    zd = z.double() / temperature
+    there = (i >= 0) & (i < z.shape[-1])
+    td = (t.double() / temperature).masked_fill(~there, float("-inf"))
+    counted = (td > float("-inf")).any(-1)
+    p = torch.where(counted[:, None], torch.softmax(td, -1), torch.zeros_like(td))
+    place = i.long().clamp(0, z.shape[-1] - 1)
+    log_q = torch.log_softmax(zd, -1)
+    terms = torch.where(p > 0, torch.special.xlogy(p, p) - p * log_q.gather(-1, place), torch.zeros_like(p))
+    q = log_q.exp()
+    grad = torch.where(counted[:, None], q, torch.zeros_like(q)).scatter_add(-1, place, -p)
+    return terms.sum(-1) * temperature ** 2, grad * temperature, counted, q, torch.zeros_like(q).scatter_add(-1, place, p), (p * log_q.gather(-1, place).abs().nan_to_num(0, 0, 0)).sum(-1)
+
+
+def _check(z, t, i, temperature=1.0, reduction="mean", both=True):
+    vocab = z.shape[-1]
+    loss_rows, dz, counted, q, p, size = _oracle(z.detach(), t, i, temperature)
+    x = (z.double() / temperature - (z.double() / temperature).amax(-1, keepdim=True)).nan_to_num(0, 0, 0).abs() * 1.4427
+    far = x.clamp_max(60).amax(-1)                     # (2^-60 and less is nothing)
+    slack = 4 * U + 2 * U * far + (vocab / 32 + 64) * U
+    rows = max(1, int(counted.sum()))
+    divisor = rows if reduction == "mean" else 1
+    leaf = z.detach().requires_grad_()
+    loss = sa.distillation_loss(leaf, t, i, temperature=temperature, reduction=reduction)
+    assert loss.dtype == torch.float32
+    per_row = temperature ** 2 * slack * (1 + 0 * size) + 4 * U * (loss_rows.abs() + temperature ** 2 * size)
+    per_row = torch.where(counted, per_row, torch.zeros_like(per_row))
+    want = loss_rows if reduction == "none" else loss_rows.sum() / divisor
+    bound = per_row if reduction == "none" else per_row.sum() / divisor + 2 * U * want.abs()
+    assert ((loss.double() - want).abs() <= bound).all()
+
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    gout = torch.rand(loss.shape, generator=gen, device="cuda") + 0.5
+    got = torch.autograd.grad(loss, leaf, gout)[0]
+    assert got.dtype == z.dtype and got.shape == z.shape
+    if reduction != "none":
+        gout = gout.expand(z.shape[0])
+
+    def grad_close(got, g):
+        g = g.double()[:, None] / divisor
+        bound = g.abs() * temperature * (q * (2 * slack + 2 * U * x + 8 * U)[...] + p * 1032 * U) + (dz * g).abs() * _half_step(z) * (1 + 2 ** -7) + 2.0 ** -133
+        assert ((got.double() - dz * g).abs() <= bound).all()
+
+    slack = slack[:, None]
+    grad_close(got, gout)
+    assert (got[~counted] == 0).all()
+    if both and reduction != "none":
+        one, grad = sa.distillation_loss_and_grad(z.detach(), t, i, temperature=temperature, reduction=reduction, grad_scale=3.0)
+        assert ((one.double() - want).abs() <= bound).all()
+        grad_close(grad, torch.full_like(gout, 3.0))
+        assert (grad[~counted] == 0).all()
+    return loss, got
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("rows, vocab, k, temperature", [
+    (1, 1, 1, 1.0), (3, 2, 5, 0.5), (17, 7, 3, 2.0), (9, 256, 8, 1.0), (33, 255, 16, 1.5), (8, 2048, 64, 1.0), (5, 2049, 64, 3.0), (70, 4097, 33, 1.0),
+    (3, 32000, 100, 2.0), (2, 50257 + 1, 1024, 1.0), (1, 131071, 1, 0.7), (4, 128000, 64, 2.0), (2, 262145, 20, 1.0), (1, 700001, 9, 4.0),
+], ids=str)
+def test_against_64_bits(rows, vocab, k, temperature, dtype):
+    z, t, i = _inputs(rows, vocab, k, dtype)
+    _check(z, t, i, temperature)
+
+
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+@pytest.mark.parametrize("vocab", [300, 5003, 40000])
+def test_reductions_and_absent_entries(reduction, vocab):
+    z, t, i = _inputs(13, vocab, 12, torch.float32, torch.bfloat16)
+    i[2] = -1                                # no teacher
+    i[5, 3:] = -1
+    t[5, 3:] = float("nan")                  # ... whatever stands there
+    i[6, ::2] = vocab + 7
+    i[7, 1:] = i[7, 0]                       # one token alone
+    i[8, 6:] = i[8, :6]                      # tokens twice
+    t[9, 4:] = float("-inf")
+    t[10] = float("-inf")                    # no mass
+    t[11, 2] = torch.finfo(torch.bfloat16).min
+    i[12, 1:] = -5
+    i[12, 0] = vocab - 1
+    _check(z, t, i, 1.7, reduction)
+    _check(z, t, i.int(), 1.7, reduction)
+    _check(z[:3], t[10:11].expand(3, 12), i[:3], 1.0, reduction)             # no row counts
+
+
+@pytest.mark.parametrize("vocab", [64, 3001, 90000])
+def test_masked_students(vocab):
+    z, t, i = _inputs(6, vocab, 5, torch.float32)
+    i = (torch.arange(5, device="cuda") * 3 + torch.arange(6, device="cuda")[:, None]).contiguous()
+    z[0, 40:] = float("-inf")                # tokens that are out of the question
+    z[1, 41:] = torch.finfo(torch.float32).min
+    z[2] = 1e4 * z[2]
+    z[3] = z[3] + 3e4
+    z[4] = 0.0
+    _check(z, t, i, 2.0, "none")
+    _check(z, t, i, 2.0, "mean")
+    # the teacher wants what the student rules out
+    z[0, i[0, 0]] = float("-inf")
+    assert sa.distillation_loss(z, t, i, reduction="none")[0] == float("inf")
+    # NaN stays in its row
+    z[5, 63] = float("nan")
+    loss = sa.distillation_loss(z, t, i, reduction="none")
+    assert loss[5].isnan() and not loss[1:5].isnan().any()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("vocab", [100, 2500, 60001])
+def test_strided_rows_and_shapes(vocab, dtype):
+    z, t, i = _inputs(6, vocab + 3, 4, dtype)
+    i.clamp_(max=vocab - 1)
+    i[:, 1:] = torch.where(i[:, 1:] == i[:, :1], torch.full_like(i[:, 1:], -1), i[:, 1:])
+    for view in (z[:, 1:vocab + 1], z[:, 3:], z[::2, :vocab], z[:, :vocab].t().contiguous().t()):
+        m = view.shape[0]
+        _check(view, t[:m], i[:m], 1.0)
+    _check(z[:, :vocab], torch.cat((t, t), 1)[:, 1:5], torch.cat((i, i), 1)[:, 1:5], 1.0)
+    three = z.view(2, 3, -1)[..., :vocab]
+    leaf = three.detach().requires_grad_()
+    a = sa.distillation_loss(leaf, t.view(2, 3, 4), i.view(2, 3, 4), reduction="none")
+    assert a.shape == (2, 3)
+    # the order of a row's sum follows its 16-byte boundaries: both are within the bound of _check, whose exponents stay below 60 here
+    packed = sa.distillation_loss(z[:, :vocab].contiguous(), t, i, reduction="none")
+    assert ((a.flatten() - packed).abs() <= 2 * ((4 + 2 * 60 + vocab / 32 + 64) * U + 4 * U * (packed.abs() + 60))).all()
+    grad = torch.autograd.grad(a.sum(), leaf)[0]
+    assert grad.shape == three.shape
+    one, g = sa.distillation_loss_and_grad(three, t.view(2, 3, 4), i.view(2, 3, 4), reduction="sum")
+    assert one.shape == () and g.shape == three.shape
+    # one row without a batch
+    assert torch.equal(sa.distillation_loss(three[1, 2], t[5], i[5], reduction="none"), a[1, 2])
+
+
+def test_nothing():
+    z, t, i = torch.zeros(0, 7, device="cuda"), torch.zeros(0, 2, device="cuda"), torch.zeros(0, 2, dtype=torch.long, device="cuda")
+    leaf = z.requires_grad_()
+    loss = sa.distillation_loss(leaf, t, i)
+    assert loss == 0 and torch.autograd.grad(loss, leaf)[0].shape == (0, 7)
+    loss, grad = sa.distillation_loss_and_grad(z.detach(), t, i)
+    assert loss == 0 and grad.shape == (0, 7)
+
+
+def test_gradient_against_differences():
+    """A step to either side along a direction; what the step misses comes from the oracle, roundings are bounded as above."""
+    z, t, i = _inputs(5, 900, 6, torch.float32)
+    leaf = z.requires_grad_()
+    loss, grad = _check(z, t, i, 1.3, "sum")
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    way = torch.randn(z.shape, generator=gen, device="cuda")
+    h = 2.0 ** -6
+    sides = [(leaf.detach() + s * h * way) for s in (1, -1)]
+    loss = sa.distillation_loss(leaf, t, i, temperature=1.3, reduction="sum")
+    slope = (torch.autograd.grad(loss, leaf)[0].double() * way.double()).sum()
+    apart = [sa.distillation_loss(x, t, i, temperature=1.3, reduction="none").double().sum() for x in sides]
+    exact = [_oracle(x, t, i, 1.3)[0].sum() for x in sides]
+    true = (_oracle(leaf.detach(), t, i, 1.3)[1] * way.double()).sum()
+    missed = ((exact[0] - exact[1]) / (2 * h) - true).abs()
+    rounding = 5 * 1.3 ** 2 * (4 + 2 * 40 + 900 / 32 + 64 + 100) * U / h
+    assert ((apart[0] - apart[1]) / (2 * h) - slope).abs() <= missed + rounding
+    assert missed + rounding <= 0.05 * grad.double().norm() * way.double().norm()
+
+
+@pytest.mark.parametrize("vocab", [256, 20000])
+def test_same_bits_streams_and_captured(vocab):
+    z, t, i = _inputs(300, vocab, 16, torch.bfloat16)
+    leaf = z.detach().clone().requires_grad_()
+
+    def step():
+        loss = sa.distillation_loss(leaf, t, i, temperature=2.0)
+        return [loss.detach(), *torch.autograd.grad(loss, leaf), *sa.distillation_loss_and_grad(leaf.detach(), t, i, temperature=2.0)]
+
+    first = step()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for a, b in zip(first, step()):
+            assert torch.equal(a, b)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        res = step()
+    with torch.no_grad():
+        t.normal_()
+        leaf.normal_()
+    i.random_(0, vocab)
+    graph.replay()
+    for a, b in zip(res, step()):
+        assert torch.equal(a, b)
+
+
+def test_the_loss_is_the_callers_and_no_second_backward():
+    z, t, i = _inputs(4, 100, 3, torch.float32)
+    leaf = z.requires_grad_()
+    loss = sa.distillation_loss(leaf, t, i)
+    want = torch.autograd.grad(loss, leaf, retain_graph=True)[0]
+    loss.data.zero_()
+    assert torch.equal(torch.autograd.grad(loss, leaf, retain_graph=True)[0], want)
+    with pytest.raises(RuntimeError, match="create_graph"):
+        torch.autograd.grad(loss, leaf, create_graph=True)
