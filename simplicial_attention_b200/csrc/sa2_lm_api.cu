@@ -211,6 +211,20 @@ template <typename T> int distill_bwd(const sa2_distill_args *a) {
     return launch_status();
 }
 
+// ---------------------------------------------------------------- sampling
+template <typename T, bool RESIDENT, int N> int sample_launch(const sa2::sample::Params &P, int ctas, cudaStream_t st) {
+    using namespace sa2::sample;
+    const size_t behind = RESIDENT ? (size_t)P.slice : (size_t)WARPS<N> * RING * 128;
+    return launch_clusters(kernel<T, RESIDENT, N>, P.rows * ctas, N, sizeof(Shared<N>) + behind * sizeof(T), ctas, st, P);
+}
+template <typename T> int sample_run(const sa2::sample::Params &P, int ctas, cudaStream_t st) {
+    // many short rows: small CTAs, whose waits overlap
+    if (ctas == 1 && P.vocab <= sa2::sample::SHORT && P.rows > SM_COUNT) return sample_launch<T, true, 128>(P, ctas, st);
+    // two CTAs an SM; rows that do not fit are read from memory again
+    if (sizeof(sa2::sample::Shared<512>) + (size_t)P.slice * sizeof(T) <= 112 * 1024) return sample_launch<T, true, 512>(P, ctas, st);
+    return sample_launch<T, false, 512>(P, ctas, st);
+}
+
 }  // namespace
 
 extern "C" {
@@ -280,16 +294,11 @@ int sa2_sample(const sa2_sample_args *a) {
     P.token = a->token; P.logprob = a->logprob; P.rows = a->rows; P.zs = a->logits_stride;
     P.top_k_all = a->top_k_all; P.temperature_all = a->temperature_all; P.top_p_all = a->top_p_all; P.min_p_all = a->min_p_all;
     P.vocab = a->vocab; P.uniform64 = a->uniform64;
-    const int size = size_of(a->dtype), ctas = sm::ctas_of(a->rows, a->vocab, size, SM_COUNT);
+    const int ctas = sm::ctas_of(a->rows, a->vocab, SM_COUNT);
     P.slice = sm::slice_of(a->vocab, ctas);
     P.shift = sm::mass_shift(a->vocab);
-    size_t smem = sizeof(sm::Shared) + (size_t)P.slice * size;
-    P.resident = smem <= 200 * 1024;
-    if (!P.resident) smem = sizeof(sm::Shared);
     if (a->rows * ctas > INT32_MAX) return SA2_ERR_UNSUPPORTED;
-    cudaStream_t st = stream_of(a->stream);
-    return a->dtype == SA2_BF16 ? launch_clusters(sm::kernel<__nv_bfloat16>, a->rows * ctas, sm::THREADS, smem, ctas, st, P)
-                                : launch_clusters(sm::kernel<float>, a->rows * ctas, sm::THREADS, smem, ctas, st, P);
+    return a->dtype == SA2_BF16 ? sample_run<__nv_bfloat16>(P, ctas, stream_of(a->stream)) : sample_run<float>(P, ctas, stream_of(a->stream));
 }
 
 }  // extern "C"
