@@ -379,17 +379,19 @@ size_t sa2_embed_workspace_bytes(int64_t rows, int32_t dim);
  *   loss[r] = T^2 sum_k p_k (log p_k - log q[index_k]),   dlogits_j = g T (q_j - sum of p_k over index_k == j)
  * Entries with an index outside [0, vocab) are not there; a row without entries (or with none above -inf) has loss and gradient
  * zero.  Rows are strided, their elements contiguous; logits and dlogits fp32 or bf16 (dtype), teacher fp32 or bf16, index int64 or int32.
- * sa2_distill_fwd writes row_loss, stats [rows][2] and counted, and total[2]: the sum of row_loss over `reduction` (SA2_SUM: 1,
- * SA2_MEAN: the number of rows with entries, at least 1), and one over that divisor.  sa2_distill_bwd reads stats and total[1], and gout: the gradient of the
- * total, or of every row (gout_rows != 0); null is 1.  sa2_distill_both is the forward and the backward for gout = grad_scale.
+ * sa2_distill_fwd writes row_loss, and total: the sum of row_loss over `reduction` (SA2_SUM: 1, SA2_MEAN: the number of rows with
+ * entries, at least 1); either may be null.  The workspace (sa2_distill_workspace_bytes(), 256-byte aligned) keeps what sa2_distill_bwd needs
+ * beside the logits; gout is the gradient of the total, or of every row (gout_rows != 0), null is 1.  sa2_distill_both is the forward and
+ * the backward for gout = grad_scale, which reads the logits from memory once.
  */
 typedef enum sa2_reduction { SA2_SUM = 0, SA2_MEAN = 1 } sa2_reduction;
 typedef struct sa2_distill_args {
-    const void *logits, *teacher, *index;
-    float *row_loss, *stats, *total;
-    int32_t *counted;
-    const float *gout;
+    const void *logits, *teacher, *index;   /* teacher, index: forward only */
+    float *row_loss, *total;                /* forward only */
+    const float *gout;                      /* backward only */
     void *dlogits;
+    void *workspace;
+    size_t workspace_bytes;
     int64_t rows, logits_stride, teacher_stride, index_stride, dlogits_stride;
     int32_t vocab, k, dtype, teacher_dtype, index64, reduction, gout_rows;
     float temperature, grad_scale;
@@ -399,6 +401,7 @@ typedef struct sa2_distill_args {
 int sa2_distill_fwd(const sa2_distill_args *args);
 int sa2_distill_bwd(const sa2_distill_args *args);
 int sa2_distill_both(const sa2_distill_args *args);
+size_t sa2_distill_workspace_bytes(int64_t rows, int32_t k);
 
 /*
  * One token for each row of logits (fp32 or bf16, element stride 1): temperature, then the first top_k, then those before which less

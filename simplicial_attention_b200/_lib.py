@@ -25,7 +25,7 @@ EXPORTS = ("sa2_fwd", "sa2_bwd", "sa2_bwd_workspace_bytes", "sa2_strerror", "sa2
            "sa2_norm_linear", "sa2_step_attn",
            "sa2_rotary_fwd", "sa2_rotary_bwd", "sa2_rotary_partial_bytes",
            "sa2_embed_fwd", "sa2_embed_bwd", "sa2_embed_workspace_bytes",
-           "sa2_distill_fwd", "sa2_distill_bwd", "sa2_distill_both", "sa2_sample")
+           "sa2_distill_fwd", "sa2_distill_bwd", "sa2_distill_both", "sa2_distill_workspace_bytes", "sa2_sample")
 STATIC_SCRATCH_ROWS = 262144   # SA2_STATIC_SCRATCH_ROWS in include/sa2.h
 SELFTEST_WAIT_BIT = 0x10000    # SA2_SELFTEST_WAIT_BIT
 SA2_ERR_DEVICE = 5

@@ -162,43 +162,38 @@ template <typename T> int embed_bwd(const sa2_embed_args *a) {
 
 // ---------------------------------------------------------------- distillation
 int distill_check(const sa2_distill_args *a, bool forward, bool backward) {
-    if (!a || !a->logits || !a->teacher || !a->index || !a->stats || !a->total || a->rows <= 0 || a->vocab <= 0 || a->k <= 0) return SA2_ERR_INVALID;
-    if (forward && (!a->row_loss || !a->counted)) return SA2_ERR_INVALID;
+    if (!a || !a->logits || a->rows <= 0 || a->vocab <= 0 || a->k <= 0) return SA2_ERR_INVALID;
+    if (forward && (!a->teacher || !a->index || (!a->row_loss && !a->total))) return SA2_ERR_INVALID;
     if (backward && !a->dlogits) return SA2_ERR_INVALID;
     if (!known(a->dtype) || !known(a->teacher_dtype) || a->k > sa2::distill::MAX_K || a->rows > INT32_MAX) return SA2_ERR_UNSUPPORTED;
     if (a->reduction != SA2_SUM && a->reduction != SA2_MEAN) return SA2_ERR_UNSUPPORTED;
     if (!(a->temperature > 0.f) || a->temperature * 0.f != 0.f) return SA2_ERR_INVALID;
     const uintptr_t unit = size_of(a->dtype) - 1;
     if ((reinterpret_cast<uintptr_t>(a->logits) & unit) || (backward && (reinterpret_cast<uintptr_t>(a->dlogits) & unit))) return SA2_ERR_INVALID;
+    if (!a->workspace || (reinterpret_cast<uintptr_t>(a->workspace) & 255u) || a->workspace_bytes < sa2_distill_workspace_bytes(a->rows, a->k))
+        return SA2_ERR_WORKSPACE;
     return SA2_OK;
 }
 
 sa2::distill::Params distill_params(const sa2_distill_args *a) {
     sa2::distill::Params P{};
-    P.z = a->logits; P.teacher = a->teacher; P.index = a->index; P.stats = a->stats; P.row_loss = a->row_loss; P.counted = a->counted;
+    P.z = a->logits; P.teacher = a->teacher; P.index = a->index;
     P.dz = a->dlogits; P.gout = a->gout; P.gs = a->gout_rows != 0;
-    P.scale = a->reduction == SA2_MEAN && !a->gout_rows ? a->total + 1 : nullptr;
+    P.mean = a->reduction == SA2_MEAN;
     P.times = a->grad_scale;
     P.rows = a->rows; P.zs = a->logits_stride; P.ts = a->teacher_stride; P.is = a->index_stride; P.ds = a->dlogits_stride;
     P.vocab = a->vocab; P.k = a->k; P.index64 = a->index64; P.teacher_bf16 = a->teacher_dtype == SA2_BF16; P.t = a->temperature;
+    sa2::distill::carve(P, a->workspace);
+    if (a->row_loss) P.row_loss = a->row_loss;
     return P;
 }
 
 // a warp a row up to this vocabulary
 constexpr int WARP_VOCAB = 2048;
 
-template <typename T> int distill_fwd(const sa2_distill_args *a) {
-    const sa2::distill::Params P = distill_params(a);
-    cudaStream_t st = stream_of(a->stream);
-    if (a->vocab <= WARP_VOCAB) sa2::distill::fwd_kernel<T, 32><<<(unsigned)((a->rows + 7) / 8), 256, 0, st>>>(P);
-    else sa2::distill::fwd_kernel<T, 512><<<(unsigned)a->rows, 512, 0, st>>>(P);
-    if (int e = launch_status()) return e;
-    sa2::distill::total_kernel<<<1, 1024, 0, st>>>(a->row_loss, a->counted, a->rows, a->reduction == SA2_MEAN, a->total);
-    return launch_status();
-}
-
 template <typename T> int distill_bwd(const sa2_distill_args *a) {
-    const sa2::distill::Params P = distill_params(a);
+    sa2::distill::Params P = distill_params(a);
+    if (!P.mean || a->gout_rows) P.scale = nullptr;
     cudaStream_t st = stream_of(a->stream);
     const size_t entries = (size_t)a->k * 8;
     if (a->vocab <= WARP_VOCAB) {
@@ -209,6 +204,25 @@ template <typename T> int distill_bwd(const sa2_distill_args *a) {
         sa2::distill::bwd_kernel<T, 512><<<(unsigned)a->rows, 512, entries, st>>>(P);
     }
     return launch_status();
+}
+
+// The forward; with `grad` also the gradient.
+template <typename T> int distill_fwd(const sa2_distill_args *a, bool grad) {
+    const sa2::distill::Params P = distill_params(a);
+    cudaStream_t st = stream_of(a->stream);
+    using namespace sa2::distill;
+    teacher_kernel<<<(unsigned)teacher_blocks(a->rows), 32 * TEACHER_ROWS, 0, st>>>(P);
+    if (int e = launch_status()) return e;
+    const bool both = grad && a->vocab > WARP_VOCAB;
+    if (both) both_kernel<T, 512><<<(unsigned)a->rows, 512, (size_t)a->k * 8, st>>>(P);
+    else if (a->vocab <= WARP_VOCAB) fwd_kernel<T, 32><<<(unsigned)((a->rows + 7) / 8), 256, 0, st>>>(P);
+    else fwd_kernel<T, 512><<<(unsigned)a->rows, 512, 0, st>>>(P);
+    if (int e = launch_status()) return e;
+    if (a->total) {
+        total_kernel<<<1, 1024, 0, st>>>(P.row_loss, P.counts, a->rows, P.mean, a->total, P.scale);
+        if (int e = launch_status()) return e;
+    }
+    return grad && !both ? distill_bwd<T>(a) : SA2_OK;
 }
 
 // ---------------------------------------------------------------- sampling
@@ -265,10 +279,13 @@ int sa2_embed_bwd(const sa2_embed_args *a) {
     return a->dtype == SA2_BF16 ? embed_bwd<__nv_bfloat16>(a) : embed_bwd<float>(a);
 }
 
+size_t sa2_distill_workspace_bytes(int64_t rows, int32_t k) {
+    return rows > 0 && k > 0 ? sa2::distill::workspace_bytes(rows, k) : 0;
+}
 int sa2_distill_fwd(const sa2_distill_args *a) {
     Range range("sa2_distill_fwd");
     if (int e = distill_check(a, true, false)) return e;
-    return a->dtype == SA2_BF16 ? distill_fwd<__nv_bfloat16>(a) : distill_fwd<float>(a);
+    return a->dtype == SA2_BF16 ? distill_fwd<__nv_bfloat16>(a, false) : distill_fwd<float>(a, false);
 }
 int sa2_distill_bwd(const sa2_distill_args *a) {
     Range range("sa2_distill_bwd");
@@ -278,9 +295,8 @@ int sa2_distill_bwd(const sa2_distill_args *a) {
 int sa2_distill_both(const sa2_distill_args *a) {
     Range range("sa2_distill_both");
     if (int e = distill_check(a, true, true)) return e;
-    if (a->gout) return SA2_ERR_INVALID;
-    if (int e = a->dtype == SA2_BF16 ? distill_fwd<__nv_bfloat16>(a) : distill_fwd<float>(a)) return e;
-    return a->dtype == SA2_BF16 ? distill_bwd<__nv_bfloat16>(a) : distill_bwd<float>(a);
+    if (a->gout || !a->total) return SA2_ERR_INVALID;
+    return a->dtype == SA2_BF16 ? distill_fwd<__nv_bfloat16>(a, true) : distill_fwd<float>(a, true);
 }
 
 int sa2_sample(const sa2_sample_args *a) {

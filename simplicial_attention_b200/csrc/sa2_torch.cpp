@@ -44,6 +44,7 @@ struct Lib {
     int (*distill_fwd)(const sa2_distill_args *) = nullptr;
     int (*distill_bwd)(const sa2_distill_args *) = nullptr;
     int (*distill_both)(const sa2_distill_args *) = nullptr;
+    size_t (*distill_workspace)(int64_t, int32_t) = nullptr;
     int (*sample)(const sa2_sample_args *) = nullptr;
 } L;
 
@@ -55,7 +56,7 @@ void bind(const std::map<std::string, uintptr_t> &f) {
     set(L.norm_linear, "sa2_norm_linear"); set(L.step_attn, "sa2_step_attn");
     set(L.rotary_fwd, "sa2_rotary_fwd"); set(L.rotary_bwd, "sa2_rotary_bwd"); set(L.rotary_partial, "sa2_rotary_partial_bytes");
     set(L.embed_fwd, "sa2_embed_fwd"); set(L.embed_bwd, "sa2_embed_bwd"); set(L.embed_workspace, "sa2_embed_workspace_bytes");
-    set(L.distill_fwd, "sa2_distill_fwd"); set(L.distill_bwd, "sa2_distill_bwd"); set(L.distill_both, "sa2_distill_both");
+    set(L.distill_fwd, "sa2_distill_fwd"); set(L.distill_bwd, "sa2_distill_bwd"); set(L.distill_both, "sa2_distill_both"); set(L.distill_workspace, "sa2_distill_workspace_bytes");
     set(L.sample, "sa2_sample");
 }
 
@@ -654,50 +655,45 @@ pybind11::object embed(const Tensor &tokens, const Tensor &weight, const std::op
 // reduction: SA2_SUM, SA2_MEAN, or 2 for none
 constexpr int64_t NONE = 2;
 struct Distill : torch::autograd::Function<Distill> {
-    static void fill(sa2_distill_args &a, const Tensor &logits, const Tensor &teacher, const Tensor &index, const Tensor &stats, const Tensor &total, double t, int64_t reduction) {
-        a.logits = logits.data_ptr(); a.teacher = teacher.data_ptr(); a.index = index.data_ptr();
-        a.stats = stats.data_ptr<float>(); a.total = total.data_ptr<float>();
-        a.rows = logits.size(0); a.logits_stride = logits.stride(0); a.teacher_stride = teacher.stride(0); a.index_stride = index.stride(0);
-        a.vocab = (int32_t)logits.size(1); a.k = (int32_t)teacher.size(1);
-        a.dtype = dtype_of(logits); a.teacher_dtype = dtype_of(teacher); a.index64 = index.scalar_type() == at::kLong;
-        a.reduction = reduction == SA2_MEAN ? SA2_MEAN : SA2_SUM; a.temperature = (float)t; a.grad_scale = 1.f; a.stream = stream_of(logits);
+    static void fill(sa2_distill_args &a, const Tensor &logits, const Tensor &ws, int64_t k, double t, int64_t reduction) {
+        a.logits = logits.data_ptr(); a.workspace = ws.data_ptr(); a.workspace_bytes = (size_t)ws.numel();
+        a.rows = logits.size(0); a.logits_stride = logits.stride(0); a.vocab = (int32_t)logits.size(1); a.k = (int32_t)k;
+        a.dtype = dtype_of(logits); a.reduction = reduction == SA2_MEAN ? SA2_MEAN : SA2_SUM; a.temperature = (float)t; a.grad_scale = 1.f;
+        a.stream = stream_of(logits);
     }
     static Tensor flat(const Tensor &t) {
         const Tensor r = t.dim() == 2 ? t : t.reshape({-1, t.size(-1)});
         return r.stride(1) == 1 || r.size(1) == 1 ? r : r.contiguous();
     }
-    // loss and the statistics of the rows; with `grad` also the gradient times `grad_scale`
-    static Tensor run(const Tensor &z, const Tensor &teacher, const Tensor &index, double t, int64_t reduction, Tensor &stats, Tensor &total, const Tensor &grad, double grad_scale) {
-        const auto f32 = z.options().dtype(at::kFloat);
-        const int64_t rows = z.size(0);
-        stats = at::empty({rows, 2}, f32);
-        total = at::empty({2}, f32);
-        const Tensor losses = at::empty({rows}, f32), counted = at::empty({rows}, z.options().dtype(at::kInt));
-        if (rows == 0) {
-            total.zero_();
+    // the loss, and in `ws` what the backward needs; with `grad` also the gradient times `grad_scale`
+    static Tensor run(const Tensor &z, const Tensor &teacher, const Tensor &index, double t, int64_t reduction, Tensor &ws, const Tensor &grad, double grad_scale) {
+        const int64_t rows = z.size(0), k = teacher.size(1);
+        Tensor loss = at::empty(reduction == NONE ? at::IntArrayRef{rows} : at::IntArrayRef{}, z.options().dtype(at::kFloat));
+        ws = at::empty({(int64_t)std::max<size_t>(L.distill_workspace(rows, (int32_t)k), 256)}, z.options().dtype(at::kByte));
+        if (rows == 0) return loss.zero_();
+        sa2_distill_args a{};
+        fill(a, z, ws, k, t, reduction);
+        a.teacher = teacher.data_ptr(); a.index = index.data_ptr(); a.teacher_stride = teacher.stride(0); a.index_stride = index.stride(0);
+        a.teacher_dtype = dtype_of(teacher); a.index64 = index.scalar_type() == at::kLong;
+        (reduction == NONE ? a.row_loss : a.total) = loss.data_ptr<float>();
+        a.grad_scale = (float)grad_scale;
+        if (grad.defined()) {
+            a.dlogits = grad.data_ptr(); a.dlogits_stride = grad.stride(0);
+            check(L.distill_both(&a), "sa2_distill_both");
         } else {
-            sa2_distill_args a{};
-            fill(a, z, teacher, index, stats, total, t, reduction);
-            a.row_loss = losses.data_ptr<float>(); a.counted = counted.data_ptr<int32_t>(); a.grad_scale = (float)grad_scale;
-            if (grad.defined()) {
-                a.dlogits = grad.data_ptr(); a.dlogits_stride = grad.stride(0);
-                check(L.distill_both(&a), "sa2_distill_both");
-            } else {
-                check(L.distill_fwd(&a), "sa2_distill_fwd");
-            }
+            check(L.distill_fwd(&a), "sa2_distill_fwd");
         }
-        return reduction == NONE ? losses : total.select(0, 0);
+        return loss;
     }
     static Tensor forward(AutogradContext *ctx, const Tensor &logits, const Tensor &teacher, const Tensor &index, double t, int64_t reduction) {
         const c10::cuda::CUDAGuard guard(logits.device());
-        const Tensor z = flat(logits), te = flat(teacher), ix = flat(index);
-        Tensor stats, total;
-        Tensor loss = run(z, te, ix, t, reduction, stats, total, Tensor(), 1.);
-        // (a tensor of its own: the caller may write into the loss)
-        loss = reduction == NONE ? loss.view(logits.sizes().slice(0, logits.dim() - 1)) : loss.clone();
-        ctx->save_for_backward({z, te, ix, stats, total});
+        const Tensor z = flat(logits);
+        Tensor ws;
+        Tensor loss = run(z, flat(teacher), flat(index), t, reduction, ws, Tensor(), 1.);
+        if (reduction == NONE && logits.dim() != 2) loss = loss.reshape(logits.sizes().slice(0, logits.dim() - 1));
+        ctx->save_for_backward({z, ws});
+        ctx->saved_data["i"] = std::vector<int64_t>{reduction, teacher.size(-1)};
         ctx->saved_data["t"] = t;
-        ctx->saved_data["reduction"] = reduction;
         ctx->saved_data["shape"] = logits.sizes().vec();
         return loss;
     }
@@ -706,13 +702,13 @@ struct Distill : torch::autograd::Function<Distill> {
         const auto s = ctx->get_saved_variables();
         const Tensor &z = s[0];
         const c10::cuda::CUDAGuard guard(z.device());
-        const int64_t reduction = ctx->saved_data["reduction"].toInt();
+        const auto i = ctx->saved_data["i"].toIntVector();
         Tensor grad = at::empty(z.sizes(), z.options().memory_format(at::MemoryFormat::Contiguous));
         if (grad.numel()) {
             const Tensor gout = grads[0].reshape({-1}).to(at::kFloat).contiguous();
             sa2_distill_args a{};
-            fill(a, z, s[1], s[2], s[3], s[4], ctx->saved_data["t"].toDouble(), reduction);
-            a.gout = gout.data_ptr<float>(); a.gout_rows = reduction == NONE;
+            fill(a, z, s[1], i[1], ctx->saved_data["t"].toDouble(), i[0]);
+            a.gout = gout.data_ptr<float>(); a.gout_rows = i[0] == NONE;
             a.dlogits = grad.data_ptr(); a.dlogits_stride = grad.stride(0);
             check(L.distill_bwd(&a), "sa2_distill_bwd");
         }
@@ -738,8 +734,8 @@ pybind11::object distill_both(const Tensor &logits, const Tensor &teacher, const
     const c10::cuda::CUDAGuard guard(logits.device());
     const at::AutoDispatchBelowADInplaceOrView below;
     const Tensor z = Distill::flat(logits);
-    Tensor grad = at::empty(z.sizes(), z.options().memory_format(at::MemoryFormat::Contiguous)), stats, total;
-    const Tensor loss = Distill::run(z, Distill::flat(teacher), Distill::flat(index), t, reduction, stats, total, grad, grad_scale);
+    Tensor grad = at::empty(z.sizes(), z.options().memory_format(at::MemoryFormat::Contiguous)), ws;
+    const Tensor loss = Distill::run(z, Distill::flat(teacher), Distill::flat(index), t, reduction, ws, grad, grad_scale);
     return pybind11::make_tuple(loss, grad.view(logits.sizes()));
 }
 

@@ -109,7 +109,7 @@ class SampleArgs(C.Structure):
 
 
 class DistillArgs(C.Structure):
-    _fields_ = [(n, C.c_void_p) for n in ("logits", "teacher", "index", "row_loss", "stats", "total", "counted", "gout", "dlogits")] + \
+    _fields_ = [(n, C.c_void_p) for n in ("logits", "teacher", "index", "row_loss", "total", "gout", "dlogits", "workspace")] + [("workspace_bytes", C.c_size_t)] + \
         [(n, C.c_int64) for n in ("rows", "logits_stride", "teacher_stride", "index_stride", "dlogits_stride")] + \
         [(n, C.c_int32) for n in ("vocab", "k", "dtype", "teacher_dtype", "index64", "reduction", "gout_rows")] + \
         [(n, C.c_float) for n in ("temperature", "grad_scale")] + [("stream", C.c_void_p)]
@@ -157,13 +157,16 @@ def test_c_calls_of_sampling_and_distillation():
     for kw, status in [(dict(logits=0), 1), (dict(uniform=0), 1), (dict(token=0), 1), (dict(rows=0), 1), (dict(vocab=-1), 1), (dict(dtype=3), 2), (dict(logits=A + 2), 1)]:
         assert lib.sa2_sample(C.byref(SampleArgs(**{**dict(logits=A, uniform=A, token=A, rows=2, vocab=5), **kw}))) == status
     assert lib.sa2_sample(None) == 1
-    good = dict(logits=A, teacher=A, index=A, row_loss=A, stats=A, total=A, counted=A, dlogits=A, rows=3, vocab=9, k=2, temperature=1.0)
-    for kw, status in [(dict(logits=0), 1), (dict(teacher=0), 1), (dict(index=0), 1), (dict(stats=0), 1), (dict(total=0), 1), (dict(rows=0), 1), (dict(vocab=0), 1), (dict(k=0), 1),
+    good = dict(logits=A, teacher=A, index=A, row_loss=A, total=A, dlogits=A, workspace=A, workspace_bytes=1 << 20, rows=3, vocab=9, k=2, temperature=1.0)
+    for kw, status in [(dict(logits=0), 1), (dict(rows=0), 1), (dict(workspace=0), 3), (dict(workspace=A + 16), 3), (dict(workspace_bytes=300), 3), (dict(vocab=0), 1), (dict(k=0), 1),
                        (dict(k=1025), 2), (dict(dtype=5), 2), (dict(teacher_dtype=5), 2), (dict(reduction=4), 2), (dict(temperature=0.0), 1), (dict(temperature=math.inf), 1),
                        (dict(temperature=math.nan), 1), (dict(logits=A + 2), 1)]:
         a = C.byref(DistillArgs(**{**good, **kw}))
         assert lib.sa2_distill_fwd(a) == status and lib.sa2_distill_bwd(a) == status and lib.sa2_distill_both(a) == status
-    assert lib.sa2_distill_fwd(C.byref(DistillArgs(**{**good, "row_loss": 0}))) == 1
+    for kw in (dict(teacher=0), dict(index=0), dict(row_loss=0, total=0)):
+        a = C.byref(DistillArgs(**{**good, **kw}))
+        assert lib.sa2_distill_fwd(a) == 1 and lib.sa2_distill_both(a) == 1
+    assert lib.sa2_distill_both(C.byref(DistillArgs(**{**good, "total": 0}))) == 1
     assert lib.sa2_distill_bwd(C.byref(DistillArgs(**{**good, "dlogits": 0}))) == 1
     assert lib.sa2_distill_both(C.byref(DistillArgs(**{**good, "gout": A}))) == 1
     assert lib.sa2_distill_fwd(None) == 1 and lib.sa2_distill_bwd(None) == 1 and lib.sa2_distill_both(None) == 1
