@@ -62,10 +62,10 @@ sa2::rotary::Params rotary_params(const sa2_rotary_args *a) {
     P.q = side(a->q); P.k = side(a->k);
     P.freqs = a->freqs; P.positions = a->positions; P.pb = a->pos_batch; P.pn = a->pos_seq; P.start = a->start;
     P.partial = reinterpret_cast<float *>(a->partial);
-    P.rows = (int64_t)a->b * a->n;
-    P.n = a->n; P.hq = a->q.heads; P.heads = a->q.heads + a->k.heads; P.pairs = a->pairs;
-    P.tile = sa2::rotary::tile_rows(P.rows, P.heads, a->d, a->pairs, SM_COUNT);
-    P.interleaved = a->interleaved != 0; P.gain_bf16 = a->gain_dtype == SA2_BF16; P.eps = a->eps;
+    P.rows = a->b * a->n; P.n = a->n;
+    P.hq = a->q.heads; P.heads = a->q.heads + a->k.heads; P.pairs = a->pairs;
+    sa2::rotary::split(P.rows, P.heads, a->d, SM_COUNT, P.parts, P.turns);
+    P.gain_bf16 = a->gain_dtype == SA2_BF16; P.eps = a->eps;
     return P;
 }
 
@@ -73,16 +73,18 @@ template <typename T, int D> int rotary_run(const sa2::rotary::Params &P, const 
     using namespace sa2::rotary;
     cudaStream_t st = stream_of(a->stream);
     if (!backward) {
-        fwd_kernel<T, D><<<(unsigned)((P.rows + P.tile - 1) / P.tile), THREADS, fwd_smem(P.tile, P.pairs), st>>>(P);
+        const auto run = a->interleaved ? fwd_kernel<T, D, true> : fwd_kernel<T, D, false>;
+        run<<<grid((int64_t)P.rows * P.parts, FWD_CTAS<T> * SM_COUNT), THREADS, fwd_smem(P.pairs), st>>>(P);
         return launch_status();
     }
-    const int grid = bwd_grid(P.rows, P.tile, SM_COUNT);
-    bwd_kernel<T, D><<<grid, THREADS, bwd_smem(P.tile, P.pairs), st>>>(P);
+    const int ctas = grid((int64_t)P.rows * P.parts, BWD_CTAS<T> * SM_COUNT);
+    const auto run = a->interleaved ? bwd_kernel<T, D, true> : bwd_kernel<T, D, false>;
+    run<<<ctas, THREADS, bwd_smem(P.pairs), st>>>(P);
     if (int e = launch_status()) return e;
     const dim3 sums(D / 32, 2);
     if (a->gain_dtype == SA2_BF16)
-        dgain_kernel<__nv_bfloat16><<<sums, 1024, 0, st>>>(P.partial, reinterpret_cast<__nv_bfloat16 *>(a->q.dgain), reinterpret_cast<__nv_bfloat16 *>(a->k.dgain), grid, D);
-    else dgain_kernel<float><<<sums, 1024, 0, st>>>(P.partial, reinterpret_cast<float *>(a->q.dgain), reinterpret_cast<float *>(a->k.dgain), grid, D);
+        dgain_kernel<__nv_bfloat16><<<sums, 1024, 0, st>>>(P.partial, reinterpret_cast<__nv_bfloat16 *>(a->q.dgain), reinterpret_cast<__nv_bfloat16 *>(a->k.dgain), ctas, D);
+    else dgain_kernel<float><<<sums, 1024, 0, st>>>(P.partial, reinterpret_cast<float *>(a->q.dgain), reinterpret_cast<float *>(a->k.dgain), ctas, D);
     return launch_status();
 }
 
@@ -245,9 +247,9 @@ extern "C" {
 
 size_t sa2_rotary_partial_bytes(const sa2_rotary_args *a) {
     if (!a || a->b <= 0 || a->n <= 0 || a->q.heads <= 0 || a->k.heads <= 0 || a->d <= 0 || a->pairs <= 0) return 0;
-    const int64_t rows = (int64_t)a->b * a->n;
-    const int tile = sa2::rotary::tile_rows(rows, a->q.heads + a->k.heads, a->d, a->pairs, SM_COUNT);
-    return (size_t)sa2::rotary::bwd_grid(rows, tile, SM_COUNT) * 2 * a->d * sizeof(float);
+    int parts, turns;
+    sa2::rotary::split((int64_t)a->b * a->n, a->q.heads + a->k.heads, a->d, SM_COUNT, parts, turns);
+    return (size_t)sa2::rotary::grid((int64_t)a->b * a->n * parts, 3 * SM_COUNT) * 2 * a->d * sizeof(float);
 }
 int sa2_rotary_fwd(const sa2_rotary_args *a) {
     Range range("sa2_rotary_fwd");

@@ -11,10 +11,13 @@
 // product - exact for every position.  What is left of the nearest quarter turn is at most 1/8 of a turn, and its sine and
 // cosine are good to the last place of fp32, with no table to read and no limit to positions.
 //
-// Bound: reading and writing every head once.  Each (row, pair) has its sine and cosine once, in shared memory, for all heads
-// of the row; a lane holds eight channels of a head (16 bytes of bf16), the lanes of a head add their squares and exchange
-// pairs by shuffles.  The backward reads x again and forms rstd again, which costs no traffic of its own; gain gradients stay in
-// registers over all rows of a CTA, a CTA writes one partial row and a second kernel adds those in order, without atomics.
+// Bound: reading and writing every head once.  A warp has a row (or, where rows are few, a part of its heads): row, position and addresses
+// are the same for its lanes, and each sine and cosine is formed once, in shared memory of the warp, while the loads are on their way.  A lane
+// holds eight channels of a head: two groups of four, the second the partners of the first where halves are paired, so that a pair is in
+// one lane; the lanes of a head add their squares by shuffles.  A lane has the same channels in all of its heads, and their gains in registers.
+// The backward reads x again and forms rstd again, which costs no traffic of its own; gain gradients stay in registers over all rows
+// of a CTA, a CTA writes one partial row and a second kernel adds those in order, without atomics.
+// (Tiles of rows for a CTA, angles between two barriers: b16 n1024, 12 heads of 64 bf16 channels 22 us forward and 42 backward.)
 #pragma once
 #include "sa2_common.cuh"
 #include "sa2_vec8.cuh"
@@ -22,7 +25,10 @@
 namespace sa2 {
 namespace rotary {
 
-constexpr int THREADS = 256, PER_THREAD = 4;    // (row, head, eight channels) items that a thread has in flight
+constexpr int THREADS = 256, WARPS = THREADS / 32;
+// CTAs of an SM, by registers; a launch has as many, and they go on row by row
+template <typename T> constexpr int FWD_CTAS = sizeof(T) == 2 ? 4 : 3;
+template <typename T> constexpr int BWD_CTAS = sizeof(T) == 2 ? 3 : 2;
 
 struct Side {                   // queries, or keys
     const void *x, *dy;         // [b][n][h][d], element strides below
@@ -36,10 +42,10 @@ struct Params {
     const int64_t *positions;   // element strides pb, pn; null: start + row
     int64_t pb, pn, start;
     float *partial;             // backward: [gridDim.x][2][d]
-    int64_t rows;               // b * n, below 2^31
-    int n, hq, heads, pairs;    // heads: of queries and keys
-    int tile;                   // rows of a CTA at a time
-    int interleaved, gain_bf16;
+    int rows, n;                // b * n; rows of a sequence
+    int hq, heads, pairs;       // heads: of queries and keys
+    int parts, turns;           // warps of a row; what each has: heads, 256 channels at a time
+    int gain_bf16;
     float eps;
 };
 
@@ -63,181 +69,217 @@ __device__ __forceinline__ void cos_sin(int64_t position, int64_t f, float &c, f
     if (quarter == 2 || quarter == 3) s = -s;
 }
 
-// cs: cosines [tile][pairs], behind them the sines, of rows [row0, row0 + count)
-__device__ __forceinline__ void fill_angles(const Params &P, float *cs, int64_t row0, int count) {
-    for (int x = threadIdx.x; x < count * P.pairs; x += THREADS) {
-        const uint32_t row = (uint32_t)row0 + x / P.pairs, b = row / (uint32_t)P.n, i = row - b * (uint32_t)P.n;
-        const int64_t position = P.positions ? P.positions[b * P.pb + i * P.pn] : P.start + (int64_t)i;
-        cos_sin(position, P.freqs[x % P.pairs], cs[x], cs[P.tile * P.pairs + x]);
-    }
+// The channels of a lane: four from `a` on and four from `b` on.  Lanes behind the rotated channels have eight that stay.
+struct Channels { int a, b; bool turned; };
+template <bool INTERLEAVED> __device__ __forceinline__ Channels channels_of(const Params &P, int lane) {
+    const bool turned = lane * 8 < 2 * P.pairs;
+    return turned && !INTERLEAVED ? Channels{4 * lane, P.pairs + 4 * lane, true} : Channels{8 * lane, 8 * lane + 4, turned};
 }
-
-// Turns the eight channels from c0 on by `sign` times the row's angles (cos, sin: those of the row).
-__device__ __forceinline__ void turn(float (&v)[8], int c0, const Params &P, const float *cos, const float *sin, float sign) {
-    if (P.interleaved) {
-        if (c0 < 2 * P.pairs) {
+// A lane's channels as they come: they stay packed until they are used
+template <typename T> struct Raw;
+template <> struct Raw<__nv_bfloat16> {
+    uint2 a, b;
+    __device__ __forceinline__ void clear() { a = make_uint2(0u, 0u); b = a; }
+    __device__ __forceinline__ void load(const __nv_bfloat16 *p, const Channels &c) {
+        a = __ldg(reinterpret_cast<const uint2 *>(p + c.a));
+        b = __ldg(reinterpret_cast<const uint2 *>(p + c.b));
+    }
+    __device__ __forceinline__ void get(float (&v)[8]) const {
+        const uint32_t w[4] = {a.x, a.y, b.x, b.y};
 #pragma unroll
-            for (int z = 0; z < 4; ++z) {
-                const float c = cos[c0 / 2 + z], s = sign * sin[c0 / 2 + z], a = v[2 * z], b = v[2 * z + 1];
-                v[2 * z] = fmaf(a, c, -b * s);
-                v[2 * z + 1] = fmaf(b, c, a * s);
-            }
+        for (int z = 0; z < 4; ++z) {
+            v[2 * z] = __uint_as_float(w[z] << 16);
+            v[2 * z + 1] = __uint_as_float(w[z] & 0xffff0000u);
         }
+    }
+};
+template <> struct Raw<float> {
+    float4 a, b;
+    __device__ __forceinline__ void clear() { a = make_float4(0.f, 0.f, 0.f, 0.f); b = a; }
+    __device__ __forceinline__ void load(const float *p, const Channels &c) {
+        a = __ldg(reinterpret_cast<const float4 *>(p + c.a));
+        b = __ldg(reinterpret_cast<const float4 *>(p + c.b));
+    }
+    __device__ __forceinline__ void get(float (&v)[8]) const {
+        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    }
+};
+template <typename T> __device__ __forceinline__ void store44(T *p, const Channels &c, const float (&v)[8]) {
+    if constexpr (sizeof(T) == 4) {
+        *reinterpret_cast<float4 *>(p + c.a) = make_float4(v[0], v[1], v[2], v[3]);
+        *reinterpret_cast<float4 *>(p + c.b) = make_float4(v[4], v[5], v[6], v[7]);
     } else {
-        const int lane = threadIdx.x & 31, step = P.pairs / 8;          // lanes between the two channels of a pair
-        const bool first = c0 < P.pairs, on = c0 < 2 * P.pairs;
-        const int from = on ? (first ? lane + step : lane - step) : lane;
-        const int p0 = on ? (first ? c0 : c0 - P.pairs) : 0;
-        const float side = first ? -sign : sign;
+        uint32_t w[4];
 #pragma unroll
-        for (int z = 0; z < 8; ++z) {
-            const float other = __shfl_sync(0xffffffffu, v[z], from);
-            if (on) v[z] = fmaf(v[z], cos[p0 + z], side * other * sin[p0 + z]);
+        for (int z = 0; z < 4; ++z) {
+            const __nv_bfloat162 t = __floats2bfloat162_rn(v[2 * z], v[2 * z + 1]);
+            w[z] = *reinterpret_cast<const uint32_t *>(&t);
+        }
+        *reinterpret_cast<uint2 *>(p + c.a) = make_uint2(w[0], w[1]);
+        *reinterpret_cast<uint2 *>(p + c.b) = make_uint2(w[2], w[3]);
+    }
+}
+
+// Turns a lane's pairs by the angles with these cosines and sines.
+template <bool INTERLEAVED> __device__ __forceinline__ void turn(float (&v)[8], const float (&cs)[4], const float (&sn)[4]) {
+#pragma unroll
+    for (int z = 0; z < 4; ++z) {
+        float &first = INTERLEAVED ? v[2 * z] : v[z], &second = INTERLEAVED ? v[2 * z + 1] : v[4 + z];
+        const float a = first, b = second;
+        first = fmaf(a, cs[z], -b * sn[z]);
+        second = fmaf(b, cs[z], a * sn[z]);
+    }
+}
+
+__device__ __forceinline__ void load_gain(const Params &P, const void *gain, const Channels &c, float (&g)[8]) {
+    if (P.gain_bf16) {
+        Raw<__nv_bfloat16> r;
+        r.load(reinterpret_cast<const __nv_bfloat16 *>(gain), c);
+        r.get(g);
+    } else {
+        Raw<float> r;
+        r.load(reinterpret_cast<const float *>(gain), c);
+        r.get(g);
+    }
+}
+
+// A warp's unit: a row, and which of its heads
+struct Unit { int row, b, i, begin, end; };
+template <int D> __device__ __forceinline__ Unit unit_of(const Params &P, int x) {
+    Unit u;
+    u.row = P.parts == 1 ? x : x / P.parts;
+    u.b = u.row / P.n;
+    u.i = u.row - u.b * P.n;
+    const int part = x - u.row * P.parts;
+    u.begin = part * P.turns * (256 / D);
+    u.end = min(P.heads, u.begin + P.turns * (256 / D));
+    return u;
+}
+// sines and cosines of a row's position into a warp's shared memory, cosines first; then this lane's
+__device__ __forceinline__ void angles(const Params &P, const Unit &u, float *mine, int lane, bool turned, float (&cs)[4], float (&sn)[4], float sign) {
+    const int64_t position = P.positions ? P.positions[u.b * P.pb + u.i * P.pn] : P.start + u.i;
+    __syncwarp();                                        // the last row's are read
+    for (int x = threadIdx.x & 31; x < P.pairs; x += 32) cos_sin(position, P.freqs[x], mine[x], mine[P.pairs + x]);
+    __syncwarp();
+    if (turned) {
+        const float4 c = *reinterpret_cast<const float4 *>(mine + 4 * lane), t = *reinterpret_cast<const float4 *>(mine + P.pairs + 4 * lane);
+        cs[0] = c.x; cs[1] = c.y; cs[2] = c.z; cs[3] = c.w;
+        sn[0] = sign * t.x; sn[1] = sign * t.y; sn[2] = sign * t.z; sn[3] = sign * t.w;
+    }
+}
+
+template <typename T, int D, bool INTERLEAVED>
+__global__ void __launch_bounds__(THREADS, FWD_CTAS<T>) fwd_kernel(const __grid_constant__ Params P) {
+    extern __shared__ __align__(16) float shared[];
+    constexpr int LANES = D / 8, HEADS = 256 / D, U = 3;         // heads of a warp at a time; times
+    const int lane = threadIdx.x % LANES, sub = threadIdx.x % 32 / LANES, warp = threadIdx.x >> 5;
+    const Channels ch = channels_of<INTERLEAVED>(P, lane);
+    float gq[8], gk[8];
+    load_gain(P, P.q.gain, ch, gq);
+    load_gain(P, P.k.gain, ch, gk);
+    const int units = P.rows * P.parts;
+    for (int x = blockIdx.x * WARPS + warp; x < units; x += gridDim.x * WARPS) {
+        const Unit w = unit_of<D>(P, x);
+        const T *xq = reinterpret_cast<const T *>(P.q.x) + w.b * P.q.sb + w.i * P.q.sn, *xk = reinterpret_cast<const T *>(P.k.x) + w.b * P.k.sb + w.i * P.k.sn;
+        T *yq = reinterpret_cast<T *>(P.q.y) + (int64_t)w.row * P.hq * D, *yk = reinterpret_cast<T *>(P.k.y) + (int64_t)w.row * (P.heads - P.hq) * D;
+        float cs[4], sn[4];
+        for (int h0 = w.begin + sub; h0 - sub < w.end; h0 += U * HEADS) {
+            Raw<T> x0[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int h = h0 + u * HEADS;
+                x0[u].clear();
+                if (h < w.end) x0[u].load(h < P.hq ? xq + h * P.q.sh : xk + (h - P.hq) * P.k.sh, ch);
+            }
+            if (h0 - sub == w.begin) angles(P, w, shared + warp * 2 * P.pairs, lane, ch.turned, cs, sn, 1.f);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int h = h0 + u * HEADS;
+                if (h - sub >= w.end) break;
+                float v[8], ss = 0.f;
+                x0[u].get(v);
+#pragma unroll
+                for (int z = 0; z < 8; ++z) ss = fmaf(v[z], v[z], ss);
+                const float rstd = rsqrtf(head_sum<D>(ss) / (float)D + P.eps);
+#pragma unroll
+                for (int z = 0; z < 8; ++z) v[z] = v[z] * rstd * (h < P.hq ? gq[z] : gk[z]);
+                if (ch.turned) turn<INTERLEAVED>(v, cs, sn);
+                if (h < w.end) store44<T>(h < P.hq ? yq + h * D : yk + (h - P.hq) * D, ch, v);
+            }
         }
     }
 }
 
-template <int D> __device__ __forceinline__ void load_gain(const Params &P, const void *gain, int c0, float (&g)[8]) {
-    if (P.gain_bf16) load8<__nv_bfloat16>(reinterpret_cast<const __nv_bfloat16 *>(gain) + c0, g);
-    else load8<float>(reinterpret_cast<const float *>(gain) + c0, g);
-}
-
-// item of a tile: lane of the head, head of the row, row
-struct Item { int row, head, c0; bool on; };
-template <int D> __device__ __forceinline__ Item item_of(const Params &P, int x, int count) {
-    constexpr int LANES = D / 8;
-    Item t;
-    t.c0 = x % LANES * 8;
-    t.row = x / (LANES * P.heads);
-    t.head = x / LANES - t.row * P.heads;
-    t.on = t.row < count;
-    return t;
-}
-
-template <typename T, int D>
-__global__ void __launch_bounds__(THREADS) fwd_kernel(const __grid_constant__ Params P) {
-    extern __shared__ float cs[];
-    const int64_t row0 = (int64_t)blockIdx.x * P.tile;
-    const int count = (int)min((int64_t)P.tile, P.rows - row0), items = count * P.heads * (D / 8);
-    for (int base = 0; base < items; base += THREADS * PER_THREAD) {
-        float v[PER_THREAD][8];
-#pragma unroll
-        for (int u = 0; u < PER_THREAD; ++u) {
-            const Item t = item_of<D>(P, base + u * THREADS + threadIdx.x, count);
-#pragma unroll
-            for (int z = 0; z < 8; ++z) v[u][z] = 0.f;
-            if (t.on) {
-                const uint32_t row = (uint32_t)row0 + t.row, b = row / (uint32_t)P.n, i = row - b * (uint32_t)P.n;
-                const bool q = t.head < P.hq;
-                const Side &S = q ? P.q : P.k;
-                load8<T>(reinterpret_cast<const T *>(S.x) + b * S.sb + i * S.sn + (int64_t)(q ? t.head : t.head - P.hq) * S.sh + t.c0, v[u]);
-            }
-        }
-        if (base == 0) {
-            fill_angles(P, cs, row0, count);
-            __syncthreads();
-        }
-#pragma unroll
-        for (int u = 0; u < PER_THREAD; ++u) {
-            const Item t = item_of<D>(P, base + u * THREADS + threadIdx.x, count);
-            if (!__any_sync(0xffffffffu, t.on)) break;
-            float ss = 0.f;
-#pragma unroll
-            for (int z = 0; z < 8; ++z) ss = fmaf(v[u][z], v[u][z], ss);
-            const float rstd = rsqrtf(head_sum<D>(ss) / (float)D + P.eps);
-            const bool q = t.head < P.hq;
-            const Side &S = q ? P.q : P.k;
-            float g[8];
-            load_gain<D>(P, S.gain, t.c0, g);
-#pragma unroll
-            for (int z = 0; z < 8; ++z) v[u][z] = v[u][z] * rstd * g[z];
-            const float *cos = cs + (t.on ? t.row : 0) * P.pairs;
-            turn(v[u], t.c0, P, cos, cos + P.tile * P.pairs, 1.f);
-            if (t.on) {
-                const int h = q ? P.hq : P.heads - P.hq, head = q ? t.head : t.head - P.hq;
-                store8<T>(reinterpret_cast<T *>(S.y) + ((row0 + t.row) * h + head) * D + t.c0, v[u]);
-            }
-        }
-    }
-}
-
-template <typename T, int D>
-__global__ void __launch_bounds__(THREADS) bwd_kernel(const __grid_constant__ Params P) {
-    extern __shared__ float cs[];
-    constexpr int LANES = D / 8, U = 2;
-    const int c0 = threadIdx.x % LANES * 8;              // a thread has the same channels in every item
+template <typename T, int D, bool INTERLEAVED>
+__global__ void __launch_bounds__(THREADS, BWD_CTAS<T>) bwd_kernel(const __grid_constant__ Params P) {
+    extern __shared__ __align__(16) float shared[];
+    constexpr int LANES = D / 8, HEADS = 256 / D, U = sizeof(T) == 2 ? 2 : 3;
+    const int lane = threadIdx.x % LANES, sub = threadIdx.x % 32 / LANES, warp = threadIdx.x >> 5;
+    const Channels ch = channels_of<INTERLEAVED>(P, lane);
     float dq[8], dk[8], gq[8], gk[8];
 #pragma unroll
     for (int z = 0; z < 8; ++z) { dq[z] = 0.f; dk[z] = 0.f; }
-    load_gain<D>(P, P.q.gain, c0, gq);
-    load_gain<D>(P, P.k.gain, c0, gk);
-    const int64_t tiles = (P.rows + P.tile - 1) / P.tile;
-    for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-        const int64_t row0 = tile * P.tile;
-        const int count = (int)min((int64_t)P.tile, P.rows - row0), items = count * P.heads * LANES;
-        for (int base = 0; base < items; base += THREADS * U) {
-            float x[U][8], e[U][8];
+    load_gain(P, P.q.gain, ch, gq);
+    load_gain(P, P.k.gain, ch, gk);
+    const int units = P.rows * P.parts;
+    for (int x = blockIdx.x * WARPS + warp; x < units; x += gridDim.x * WARPS) {
+        const Unit w = unit_of<D>(P, x);
+        const T *xq = reinterpret_cast<const T *>(P.q.x) + w.b * P.q.sb + w.i * P.q.sn, *xk = reinterpret_cast<const T *>(P.k.x) + w.b * P.k.sb + w.i * P.k.sn;
+        const T *eq = reinterpret_cast<const T *>(P.q.dy) + w.b * P.q.db + w.i * P.q.dn, *ek = reinterpret_cast<const T *>(P.k.dy) + w.b * P.k.db + w.i * P.k.dn;
+        T *yq = reinterpret_cast<T *>(P.q.y) + (int64_t)w.row * P.hq * D, *yk = reinterpret_cast<T *>(P.k.y) + (int64_t)w.row * (P.heads - P.hq) * D;
+        float cs[4], sn[4];
+        for (int h0 = w.begin + sub; h0 - sub < w.end; h0 += U * HEADS) {
+            Raw<T> x0[U], e0[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const Item t = item_of<D>(P, base + u * THREADS + threadIdx.x, count);
-#pragma unroll
-                for (int z = 0; z < 8; ++z) { x[u][z] = 0.f; e[u][z] = 0.f; }
-                if (t.on) {
-                    const uint32_t row = (uint32_t)row0 + t.row, b = row / (uint32_t)P.n, i = row - b * (uint32_t)P.n;
-                    const bool q = t.head < P.hq;
-                    const Side &S = q ? P.q : P.k;
-                    const int64_t head = q ? t.head : t.head - P.hq;
-                    load8<T>(reinterpret_cast<const T *>(S.x) + b * S.sb + i * S.sn + head * S.sh + c0, x[u]);
-                    load8<T>(reinterpret_cast<const T *>(S.dy) + b * S.db + i * S.dn + head * S.dh + c0, e[u]);
+                const int h = h0 + u * HEADS;
+                x0[u].clear();
+                e0[u].clear();
+                if (h < w.end) {
+                    x0[u].load(h < P.hq ? xq + h * P.q.sh : xk + (h - P.hq) * P.k.sh, ch);
+                    e0[u].load(h < P.hq ? eq + h * P.q.dh : ek + (h - P.hq) * P.k.dh, ch);
                 }
             }
-            if (base == 0) {
-                __syncthreads();                         // the last tile's angles are no longer read
-                fill_angles(P, cs, row0, count);
-                __syncthreads();
-            }
+            if (h0 - sub == w.begin) angles(P, w, shared + warp * 2 * P.pairs, lane, ch.turned, cs, sn, -1.f);
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const Item t = item_of<D>(P, base + u * THREADS + threadIdx.x, count);
-                if (!__any_sync(0xffffffffu, t.on)) break;
-                float ss = 0.f;
+                const int h = h0 + u * HEADS;
+                if (h - sub >= w.end) break;
+                const bool q = h < P.hq, on = h < w.end;
+                float v[8], e[8], ss = 0.f;
+                x0[u].get(v);
+                e0[u].get(e);
 #pragma unroll
-                for (int z = 0; z < 8; ++z) ss = fmaf(x[u][z], x[u][z], ss);
+                for (int z = 0; z < 8; ++z) ss = fmaf(v[z], v[z], ss);
                 const float rstd = rsqrtf(head_sum<D>(ss) / (float)D + P.eps);
-                const float *cos = cs + (t.on ? t.row : 0) * P.pairs;
-                turn(e[u], c0, P, cos, cos + P.tile * P.pairs, -1.f);
-                const bool q = t.head < P.hq;
+                if (ch.turned) turn<INTERLEAVED>(e, cs, sn);
                 float dot = 0.f;
 #pragma unroll
                 for (int z = 0; z < 8; ++z) {
-                    x[u][z] *= rstd;
-                    const float dg = e[u][z] * x[u][z];
-                    if (t.on && q) dq[z] += dg;
-                    else if (t.on) dk[z] += dg;
-                    e[u][z] *= q ? gq[z] : gk[z];
-                    dot = fmaf(e[u][z], x[u][z], dot);
+                    v[z] *= rstd;
+                    const float dg = e[z] * v[z];
+                    if (on && q) dq[z] += dg;
+                    if (on && !q) dk[z] += dg;
+                    e[z] *= q ? gq[z] : gk[z];
+                    dot = fmaf(e[z], v[z], dot);
                 }
                 const float m = head_sum<D>(dot) / (float)D;
 #pragma unroll
-                for (int z = 0; z < 8; ++z) e[u][z] = rstd * (e[u][z] - x[u][z] * m);
-                if (t.on) {
-                    const Side &S = q ? P.q : P.k;
-                    const int h = q ? P.hq : P.heads - P.hq, head = q ? t.head : t.head - P.hq;
-                    store8<T>(reinterpret_cast<T *>(S.y) + ((row0 + t.row) * h + head) * D + c0, e[u]);
-                }
+                for (int z = 0; z < 8; ++z) e[z] = rstd * (e[z] - v[z] * m);
+                if (on) store44<T>(q ? yq + h * D : yk + (h - P.hq) * D, ch, e);
             }
         }
     }
     // the threads of a channel, in order
-    float *part = cs;                                    // [threads][8], queries and then keys
     for (int side = 0; side < 2; ++side) {
         __syncthreads();
-        store8<float>(part + threadIdx.x * 8, side ? dk : dq);
+        store8<float>(shared + threadIdx.x * 8, side ? dk : dq);
         __syncthreads();
         for (int c = threadIdx.x; c < D; c += THREADS) {
             float s = 0.f;
-            for (int t = c / 8; t < THREADS; t += LANES) s += part[t * 8 + c % 8];
-            P.partial[((int64_t)blockIdx.x * 2 + side) * D + c] = s;
+            for (int t = c / 8; t < THREADS; t += LANES) s += shared[t * 8 + c % 8];
+            const Channels at = channels_of<INTERLEAVED>(P, c / 8);
+            P.partial[((int64_t)blockIdx.x * 2 + side) * D + (c % 8 < 4 ? at.a : at.b) + c % 4] = s;
         }
     }
 }
@@ -260,20 +302,22 @@ __global__ void __launch_bounds__(1024) dgain_kernel(const float *partial, T *dq
     }
 }
 
-// Rows of a CTA: four items a thread, fewer where the rows would leave SMs without work; at most 16 KB of angles.
-inline int tile_rows(int64_t rows, int heads, int d, int pairs, int sms) {
-    int64_t t = THREADS * PER_THREAD / ((int64_t)heads * (d / 8));
-    if (t > rows / (2 * sms)) t = rows / (2 * sms);
-    if (t > 2048 / pairs) t = 2048 / pairs;
-    return t < 1 ? 1 : (int)t;
+// Warps of a row: one where there are 16 rows an SM, else as many as it takes to load all of its heads at once.
+inline void split(int64_t rows, int heads, int d, int sms, int &parts, int &turns) {
+    turns = (heads * d + 255) / 256;
+    parts = 1;
+    if (rows < 16 * (int64_t)sms && turns > 3) {
+        parts = (turns + 2) / 3;
+        turns = 3;
+    }
 }
-inline int bwd_grid(int64_t rows, int tile, int sms) {
-    const int64_t tiles = (rows + tile - 1) / tile;
-    return (int)(tiles < 4 * sms ? tiles : 4 * sms);
+inline int grid(int64_t units, int most) {
+    const int64_t want = (units + WARPS - 1) / WARPS;
+    return (int)(want < most ? want : most);
 }
-inline size_t fwd_smem(int tile, int pairs) { return (size_t)tile * pairs * 2 * sizeof(float); }
-inline size_t bwd_smem(int tile, int pairs) {
-    const size_t angles = fwd_smem(tile, pairs), sums = THREADS * 8 * sizeof(float);
+inline size_t fwd_smem(int pairs) { return (size_t)WARPS * pairs * 2 * sizeof(float); }
+inline size_t bwd_smem(int pairs) {
+    const size_t angles = fwd_smem(pairs), sums = THREADS * 8 * sizeof(float);
     return angles > sums ? angles : sums;
 }
 
