@@ -107,31 +107,38 @@ int embed_check(const sa2_embed_args *a) {
     return SA2_OK;
 }
 
-template <typename T, int V> int embed_fwd_run(const sa2::embed::Params &P, cudaStream_t st) {
+// pieces of a row: 256 channels in 16-byte accesses, or 128 one by one
+inline int embed_tiles(int dim, bool vec) { return vec ? (dim + 255) / 256 : (dim + 127) / 128; }
+
+template <typename T> int embed_fwd(const sa2_embed_args *a) {
     using namespace sa2::embed;
-    int lanes = 1;
-    while (lanes < THREADS && lanes * V < P.dim) lanes *= 2;
-    const int64_t rows = 4 * (THREADS / lanes);
-    // few rows: a CTA has a part of the channels
-    const int pieces = (P.dim + lanes * V - 1) / (lanes * V);
-    fwd_kernel<T, V><<<dim3((unsigned)((P.rows + rows - 1) / rows), (unsigned)(pieces < 64 ? pieces : 64)), THREADS, 0, st>>>(P, lanes);
+    const Params P{a->tokens, a->tokens64, a->weight, a->positions, a->out, a->rows, a->vocab, a->start, a->n, a->dim, a->scale};
+    const bool vec = a->dim % 8 == 0 && aligned16(a->weight) && aligned16(a->out) && aligned16(a->positions);
+    const int tiles = embed_tiles(a->dim, vec);
+    const int64_t ctas = ((a->rows + ROWS<T> - 1) / ROWS<T> * tiles + THREADS / 32 - 1) / (THREADS / 32);
+    if (ctas > INT32_MAX) return SA2_ERR_UNSUPPORTED;
+    const auto run = vec ? fwd_kernel<T, 8> : fwd_kernel<T, 4>;
+    run<<<(unsigned)ctas, THREADS, 0, stream_of(a->stream)>>>(P, tiles);
     return launch_status();
 }
 
-template <typename T> int embed_fwd(const sa2_embed_args *a) {
-    sa2::embed::Params P{a->tokens, a->tokens64, a->weight, a->positions, a->out, a->rows, a->vocab, a->start, a->n, a->dim, a->scale};
-    const bool vec = a->dim % 8 == 0 && aligned16(a->weight) && aligned16(a->out) && aligned16(a->positions);
-    return vec ? embed_fwd_run<T, 8>(P, stream_of(a->stream)) : embed_fwd_run<T, 1>(P, stream_of(a->stream));
-}
-
-template <typename T, int V> int embed_sum(const sa2::embed::BwdParams &P, cudaStream_t st) {
+template <typename T, int V> int embed_bwd_run(sa2::embed::BwdParams P, cudaStream_t st) {
     using namespace sa2::embed;
-    const int tiles = (P.dim + 32 * V - 1) / (32 * V);
-    const int64_t parts = P.dweight ? stretches(P.rows) : 0, units = (parts + (P.dpositions ? P.position_rows : 0)) * tiles;
-    if ((units + 7) / 8 > INT32_MAX || parts * tiles > INT32_MAX) return SA2_ERR_UNSUPPORTED;
-    sum_kernel<T, V><<<(unsigned)((units + 7) / 8), THREADS, 0, st>>>(P, parts, tiles);
+    P.tiles = embed_tiles(P.dim, V == 8);
+    const int sorting = P.dweight ? sort_ctas(P.rows) : 0, cluster = sorting ? sorting : 1;
+    // the others: a warp for 256 channels of a row of dP, and for 32 tokens' zeros; of two CTAs an SM, as many as clusters of eight
+    // find room beside the sort
+    const int64_t zeros = P.dweight ? (P.vocab + 31) / 32 : 0, adding = P.dpositions ? P.position_rows * P.tiles : 0;
+    int64_t others = ((zeros > adding ? zeros : adding) + SORT_WARPS - 1) / SORT_WARPS;
+    if (others > 216) others = 216;
+    others = (others + cluster - 1) / cluster * cluster;
+    if (int e = launch_clusters(sort_kernel<T, V>, sorting + others, SORT_THREADS, sort_smem(P.bits), cluster, st, P, sorting)) return e;
+    if (!P.dweight) return SA2_OK;
+    const int64_t parts = stretches(P.rows), units = parts * P.tiles;
+    if ((units + 7) / 8 > INT32_MAX || parts * P.tiles > INT32_MAX) return SA2_ERR_UNSUPPORTED;
+    sum_kernel<T, V><<<(unsigned)((units + 7) / 8), THREADS, 0, st>>>(P, parts);
     if (int e = launch_status()) return e;
-    if (parts > 1) join_kernel<T, V><<<(unsigned)(parts * tiles), THREADS, 0, st>>>(P, tiles);
+    if (parts > 1) join_kernel<T, V><<<(unsigned)(parts * P.tiles), THREADS, 0, st>>>(P);
     return launch_status();
 }
 
@@ -139,27 +146,20 @@ template <typename T> int embed_bwd(const sa2_embed_args *a) {
     using namespace sa2::embed;
     BwdParams P{};
     P.tokens = a->tokens; P.tokens64 = a->tokens64; P.dout = a->dout; P.dweight = a->dweight; P.dpositions = a->dpositions;
-    char *ws = reinterpret_cast<char *>(a->workspace);
-    const size_t list = up256((size_t)a->rows * 4);
-    for (int s = 0; s < 2; ++s) {
-        P.key[s] = reinterpret_cast<uint32_t *>(ws + 2 * s * list);
-        P.place[s] = reinterpret_cast<uint32_t *>(ws + (2 * s + 1) * list);
+    if (a->dweight) {
+        char *ws = reinterpret_cast<char *>(a->workspace);
+        const size_t list = up256((size_t)a->rows * 4);
+        for (int s = 0; s < 2; ++s) {
+            P.key[s] = reinterpret_cast<uint32_t *>(ws + 2 * s * list);
+            P.place[s] = reinterpret_cast<uint32_t *>(ws + (2 * s + 1) * list);
+        }
+        P.partial = reinterpret_cast<float *>(ws + 4 * list);
     }
-    P.partial = reinterpret_cast<float *>(ws + 4 * list);
     P.rows = a->rows; P.vocab = a->vocab; P.padding = a->padding; P.start = a->start; P.position_rows = a->position_rows;
     P.n = a->n; P.dim = a->dim; P.scale = a->scale;
     sort_plan(a->vocab, P.passes, P.bits);
-    P.vec = a->dim % 8 == 0 && aligned16(a->dout) && aligned16(a->dweight) && aligned16(a->dpositions);
-    cudaStream_t st = stream_of(a->stream);
-    if (!P.dweight) return P.vec ? embed_sum<T, 8>(P, st) : embed_sum<T, 1>(P, st);
-    // one cluster sorts; the others have 64 KB of zeros each to write, up to two CTAs an SM
-    const int ctas = sort_ctas(a->rows);
-    const int64_t bytes = a->vocab * a->dim * (int64_t)sizeof(T);
-    int64_t fill = (bytes + 65535) / 65536;
-    if (fill > 2 * SM_COUNT) fill = 2 * SM_COUNT;
-    fill = (fill + ctas - 1) / ctas * ctas;
-    if (int e = launch_clusters(sort_kernel, ctas + fill, SORT_THREADS, sort_smem(P.bits), ctas, st, P, bytes)) return e;
-    return P.vec ? embed_sum<T, 8>(P, st) : embed_sum<T, 1>(P, st);
+    const bool vec = a->dim % 8 == 0 && aligned16(a->dout) && aligned16(a->dweight) && aligned16(a->dpositions);
+    return vec ? embed_bwd_run<T, 8>(P, stream_of(a->stream)) : embed_bwd_run<T, 4>(P, stream_of(a->stream));
 }
 
 // ---------------------------------------------------------------- distillation

@@ -46,4 +46,29 @@ template <typename T> __device__ __forceinline__ void store8u(T *p, bool aligned
     for (int z = 0; z < 8; ++z) p[z] = (T)v[z];
 }
 
+// Eight values as they come: loads stay packed until they are used, so that many fit the registers at a time.
+template <typename T> struct Packed;
+template <> struct Packed<__nv_bfloat16> {
+    uint4 a;
+    __device__ __forceinline__ void load(const __nv_bfloat16 *p) { a = __ldg(reinterpret_cast<const uint4 *>(p)); }
+    __device__ __forceinline__ void get(float (&v)[8]) const {
+        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+        for (int z = 0; z < 4; ++z) {
+            v[2 * z] = __uint_as_float(w[z] << 16);
+            v[2 * z + 1] = __uint_as_float(w[z] & 0xffff0000u);
+        }
+    }
+};
+template <> struct Packed<float> {
+    float4 a, b;
+    __device__ __forceinline__ void load(const float *p) {
+        a = __ldg(reinterpret_cast<const float4 *>(p));
+        b = __ldg(reinterpret_cast<const float4 *>(p) + 1);
+    }
+    __device__ __forceinline__ void get(float (&v)[8]) const {
+        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    }
+};
+
 }  // namespace sa2
