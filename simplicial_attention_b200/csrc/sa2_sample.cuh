@@ -77,6 +77,12 @@ template <typename T> __device__ __forceinline__ uint32_t key_of(float z) {
     const uint32_t k = u & 0x80000000u ? ~u : u | 0x80000000u;
     return sizeof(T) == 2 ? k >> 16 : k;
 }
+// the smallest key of a logit that is at least z
+template <typename T> __device__ __forceinline__ uint32_t key_from_of(float z) {
+    if (sizeof(T) == 4) return key_of<T>(z);
+    const uint32_t k = key_of<float>(z);                 // (keys of bf16 end in zeros if positive, in ones if negative)
+    return (k & 0x80000000u ? k + 0xffffu : k) >> 16;
+}
 // the logit of a key
 template <typename T> __device__ __forceinline__ float logit_of(uint32_t key) {
     if (sizeof(T) == 2) key = key << 16 | (key & 0x8000u ? 0u : 0xffffu);
@@ -218,7 +224,7 @@ template <int N> __device__ __forceinline__ Shared<N> &of_cta(Shared<N> &S, int 
     return ctas > 1 ? *cooperative_groups::this_cluster().map_shared_rank(&S, r) : S;
 }
 
-// The keys of [from, to] in the views of all CTAs, at most N, into S.sorted, largest first.  How many there are.
+// The keys of [from, to] in the views of all CTAs into S.sorted, largest first.  How many there are; -1 if more than N.
 template <typename T, bool RESIDENT, int N> __device__ int gather(const Row<T, RESIDENT> &R, const View &V, Shared<N> &S, int ctas, uint32_t from, uint32_t to) {
     const int t = threadIdx.x;
     if (t == 0) S.taken = 0u;
@@ -236,7 +242,7 @@ template <typename T, bool RESIDENT, int N> __device__ int gather(const Row<T, R
     row_sync(ctas);
     int own[MAX_CTAS], n = 0, from_cta = 0, at = 0;
 #pragma unroll
-    for (int r = 0; r < MAX_CTAS; ++r) own[r] = r < ctas ? min((int)of_cta(S, ctas, r).taken, N) : 0;
+    for (int r = 0; r < MAX_CTAS; ++r) own[r] = r < ctas ? (int)of_cta(S, ctas, r).taken : 0;
 #pragma unroll
     for (int r = 0; r < MAX_CTAS; ++r) {
         if (t >= n && t < n + own[r]) {
@@ -245,7 +251,10 @@ template <typename T, bool RESIDENT, int N> __device__ int gather(const Row<T, R
         }
         n += own[r];
     }
-    n = min(n, N);
+    if (n > N) {
+        row_sync(ctas);
+        return -1;
+    }
     const uint32_t key = t < n ? of_cta(S, ctas, from_cta).keys[at] : 0u;
     S.all[t] = key;                                      // (0 behind the end: no logit has it)
     row_sync(ctas);                                      // nobody reads another CTA's keys any more
@@ -290,9 +299,10 @@ template <typename T, bool RESIDENT, int N>
 __device__ Cut cut_few(const Row<T, RESIDENT> &R, const View &V, Shared<N> &S, int ctas, uint32_t from, int64_t top_k, double top_p, unsigned long long least,
                        unsigned long long most, bool &sure) {
     const int t = threadIdx.x, n = gather(R, V, S, ctas, from, 0xffffffffu);
+    sure = n >= 0;
+    if (!sure) return no_cut(0ull);
     const uint32_t key = t < n ? S.sorted[t] : 0u;
     int last = top_k > 0 && top_k <= n ? (int)top_k - 1 : -1;            // the last token that stays
-    sure = true;
     if (top_p < 1.) {
         const unsigned long long m = t < n ? R.mass(logit_of<T>(key)) : 0ull;
         uint32_t cb = 0u;
@@ -621,6 +631,14 @@ __global__ void __launch_bounds__(N, 1024 / N) kernel(const __grid_constant__ Pa
     // What min-p drops anyway is in no list (but where top-p takes its part of the mass of what top-k keeps).
     const bool floored = by_floor && !(by_count && by_mass), first_list = floored && floor_key > 0u && per_warp <= 65536;
     const float floor_logit = first_list ? logit_of<T>(floor_key) : 0.f;
+    auto row_mass = [&]() {
+        unsigned long long m = 0ull;
+        for_quads(R, all_logits, [&](int, float (&v)[4]) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) m += R.mass(v[j]);
+        });
+        return row_sum(m);
+    };
     // Top-p of the whole row: a sum in fp32 says what the row's mass is to a ten thousandth, which mostly shows the cut already.  With min-p
     // the first round does without the histogram: what min-p leaves is mostly little, and holds the cut or needs none.
     const bool of_row = by_mass && !by_count, cuts = by_count || by_mass;
@@ -672,27 +690,14 @@ __global__ void __launch_bounds__(N, 1024 / N) kernel(const __grid_constant__ Pa
             }
         S.total[threadIdx.x] = c;
     }
-    auto row_mass = [&]() {
-        unsigned long long m = 0ull;
-        for_quads(R, all_logits, [&](int, float (&v)[4]) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) m += R.mass(v[j]);
-        });
-        return row_sum(m);
+    // (a temperature whose inverse is no fp32 number left that sum without meaning)
+    if (of_row && R.inv_t > 1e38) least = most = row_mass();
+    // The keys between which a cut lies, from the stretches [first, last]: of the numbers that are not outside of them, so that no more than one
+    // stretch more is between the two keys.  Margins: a logit's stretch is found in fp32.
+    auto key_from = [&](int last) {
+        return last < N - 1 ? key_from_of<T>(fmaxf(__double2float_ru((double)best - (last + 1) * width * 1.00001), -3.402823466e38f)) : 0u;
     };
-    // The keys between which a cut lies, from the stretches [first, last].  Margins: a logit's stretch is found in fp32.
-    auto key_below = [&](double logit) -> uint32_t {
-        float v = (float)logit;
-        v -= fabsf(v) * 1e-6f;
-        return v > -CUDART_INF_F ? key_of<T>(v) : 0u;
-    };
-    auto key_from = [&](int last) { return last < N - 1 ? key_below((double)best - (last + 1) * width * 1.00001) : 0u; };
-    auto key_to = [&](int first) {
-        float v = (float)((double)best - first * width * 0.99999);
-        v += fabsf(v) * 1e-6f;
-        return first > 0 ? min(best_key, key_of<T>(v)) : best_key;
-    };
-
+    auto key_to = [&](int first) { return first > 0 ? min(best_key, key_of<T>(__double2float_rd((double)best - first * width * 0.99999))) : best_key; };
     uint32_t from = floored ? floor_key : 0u, to = best_key;
     int last = floored ? floor_bin : N - 1;
     if (count) {
@@ -715,6 +720,8 @@ __global__ void __launch_bounds__(N, 1024 / N) kernel(const __grid_constant__ Pa
     }
     Cut cut = no_cut(0ull);
     for (bool exact = false; cuts; exact = true) {
+        // (not sure: by the estimate of the row's mass; if that is exact, there were too many after all)
+        if (exact && (!of_row || least == most)) near = false;
         if (of_row && (exact || !near)) least = most = row_mass();
         bool sure = true;
         if (near) {

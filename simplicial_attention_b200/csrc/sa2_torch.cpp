@@ -747,8 +747,8 @@ pybind11::object sample(const Tensor &logits, const Tensor &uniform, const std::
     if (uniform.sizes() != shape || (uniform.scalar_type() != at::kFloat && uniform.scalar_type() != at::kDouble) || logits.size(-1) == 0 || logits.size(-1) > INT32_MAX) return pybind11::none();
     const int64_t vocab = logits.size(-1), rows = logits.numel() / vocab;
     for (const auto *t : {&temperature, &top_p, &min_p})
-        if (*t && (!plain(**t, logits.device()) || (*t)->scalar_type() != at::kFloat || (*t)->numel() != rows || !(*t)->is_contiguous())) return pybind11::none();
-    if (top_k && (!plain(*top_k, logits.device()) || top_k->scalar_type() != at::kLong || top_k->numel() != rows || !top_k->is_contiguous())) return pybind11::none();
+        if (*t && (!plain(**t, logits.device()) || (*t)->scalar_type() != at::kFloat || (*t)->sizes() != shape || !(*t)->is_contiguous())) return pybind11::none();
+    if (top_k && (!plain(*top_k, logits.device()) || top_k->scalar_type() != at::kLong || top_k->sizes() != shape || !top_k->is_contiguous())) return pybind11::none();
     const c10::cuda::CUDAGuard guard(logits.device());
     const at::AutoDispatchBelowADInplaceOrView below;
     Tensor token = at::empty(shape, logits.options().dtype(at::kLong)), logprob;

@@ -15,19 +15,17 @@ from . import _lib
 _DTYPES = (torch.float32, torch.bfloat16)
 
 
-def _setting(value, off, name, rows, logits, dtype):
-    """(tensor of a value for each row, value for all): one of the two."""
-    if value is None:
-        return None, off
-    if isinstance(value, Tensor):
-        if value.is_floating_point() != dtype.is_floating_point or value.dtype == torch.bool or value.is_complex():
-            raise ValueError(f"{name}: expected {'floating-point' if dtype.is_floating_point else 'whole'} numbers, not {value.dtype}")
-        if value.shape != rows:
-            raise ValueError(f"{name}: expected a value for each row, shape {tuple(rows)}, not {tuple(value.shape)}")
-        if value.device != logits.device:
-            raise ValueError(f"{name} must be on the device of the logits")
-        return value.to(dtype).contiguous(), off
-    return None, value
+def _setting(value, name, rows, logits, dtype):
+    """A tensor of a value for each row as the kernel reads it."""
+    if not isinstance(value, Tensor):
+        return value
+    if value.is_floating_point() != dtype.is_floating_point or value.dtype == torch.bool or value.is_complex():
+        raise ValueError(f"{name}: expected {'floating-point' if dtype.is_floating_point else 'whole'} numbers, not {value.dtype}")
+    if value.shape != rows:
+        raise ValueError(f"{name}: expected a value for each row, shape {tuple(rows)}, not {tuple(value.shape)}")
+    if value.device != logits.device:
+        raise ValueError(f"{name} must be on the device of the logits")
+    return value.to(dtype).contiguous()
 
 
 def sample_tokens(logits: Tensor, uniform: Tensor, *, temperature=1.0, top_k=None, top_p=None, min_p=None, return_logprobs: bool = False):
@@ -42,20 +40,27 @@ def sample_tokens(logits: Tensor, uniform: Tensor, *, temperature=1.0, top_k=Non
 
     The result is a function of the arguments alone: the same for a row whatever the rows beside it.  A row that holds a NaN or +inf,
     or nothing above -inf, has no distribution: token -1, log-probability NaN."""
-    rows = logits.shape[:-1]
-    for name, value in (("temperature", temperature), ("top_p", top_p), ("min_p", min_p)):
-        if not isinstance(value, Tensor) and value is not None and not (math.isfinite(value) and value >= 0):
+    t, k, p, m = (None if isinstance(v, Tensor) else off if v is None else v for v, off in ((temperature, 1.0), (top_k, 0), (top_p, 1.0), (min_p, 0.0)))
+    for name, value in (("temperature", t), ("top_p", p), ("min_p", m)):
+        if value is not None and not 0 <= value < math.inf:
             raise ValueError(f"{name} must be finite and not negative, not {value}")
-    t, t_all = _setting(temperature, 1.0, "temperature", rows, logits, torch.float32)
-    k, k_all = _setting(top_k, 0, "top_k", rows, logits, torch.int64)
-    p, p_all = _setting(top_p, 1.0, "top_p", rows, logits, torch.float32)
-    m, m_all = _setting(min_p, 0.0, "min_p", rows, logits, torch.float32)
-    res = _lib.ext().sample(logits, uniform, t, float(t_all), k, int(k_all), p, float(p_all), m, float(m_all), bool(return_logprobs))
-    if res is not None:
-        return res if return_logprobs else res[0]
-    assert logits.is_cuda and uniform.is_cuda, "sample_tokens needs CUDA tensors"
-    if logits.dtype not in _DTYPES or uniform.dtype not in (torch.float32, torch.float64):
-        raise ValueError("logits must be float32 or bfloat16, uniform float32 or float64")
-    if logits.dim() < 1 or logits.shape[-1] == 0 or uniform.shape != rows:
-        raise ValueError("expected logits of (..., vocab) and a uniform number for each row")
-    raise RuntimeError("sample_tokens takes plain tensors of one device, outside of tracing and transforms")
+    numbers = (1.0 if t is None else float(t), 0 if k is None else int(k), 1.0 if p is None else float(p), 0.0 if m is None else float(m))
+
+    def call(t, k, p, m):
+        return _lib.ext().sample(logits, uniform, t, numbers[0], k, numbers[1], p, numbers[2], m, numbers[3], bool(return_logprobs))
+
+    res = call(*(v if isinstance(v, Tensor) else None for v in (temperature, top_k, top_p, min_p)))
+    if res is None:
+        # tensors of other types, or what cannot be taken
+        assert logits.is_cuda and uniform.is_cuda, "sample_tokens needs CUDA tensors"
+        if logits.dtype not in _DTYPES or uniform.dtype not in (torch.float32, torch.float64):
+            raise ValueError("logits must be float32 or bfloat16, uniform float32 or float64")
+        rows = logits.shape[:-1]
+        if logits.dim() < 1 or logits.shape[-1] == 0 or uniform.shape != rows:
+            raise ValueError("expected logits of (..., vocab) and a uniform number for each row")
+        res = call(*(v if isinstance(v, Tensor) else None for v in (
+            _setting(temperature, "temperature", rows, logits, torch.float32), _setting(top_k, "top_k", rows, logits, torch.int64),
+            _setting(top_p, "top_p", rows, logits, torch.float32), _setting(min_p, "min_p", rows, logits, torch.float32))))
+        if res is None:
+            raise RuntimeError("sample_tokens takes plain tensors of one device, outside of tracing and transforms")
+    return res if return_logprobs else res[0]

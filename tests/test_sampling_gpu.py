@@ -81,6 +81,59 @@ def test_several_ctas_a_row(rows, vocab, dtype):
         _check(z, u, **settings)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("rows, vocab", [(300, 100), (260, 129), (400, 1000), (170, 16384)], ids=str)
+def test_many_short_rows(rows, vocab, dtype):
+    """More rows than SMs: CTAs of 128 threads."""
+    z, u = _logits(rows, vocab, dtype)
+    for settings in (dict(), dict(top_k=40), dict(top_p=0.9), dict(min_p=0.05), dict(top_k=300, top_p=0.99, temperature=1.7), dict(temperature=0.0)):
+        _check(z, u, **settings)
+
+
+def test_more_rows_than_fit_and_rows_from_memory():
+    """200 rows of 128001: a CTA a row, which does not fit into shared memory and, odd, begins on no 16-byte boundary; then such that do."""
+    for vocab in (128001, 60000):
+        z, u = _logits(200, vocab, torch.float32)
+        few = slice(0, 200, 19)                          # (the oracle is slow)
+        for settings in (dict(top_p=0.6), dict(top_k=2000, top_p=0.9), dict(min_p=0.02, top_p=0.9), dict()):
+            got = sa.sample_tokens(z, u, **settings)
+            assert torch.equal(got[few].cpu(), _oracle(z[few], u[few], **settings)[0])
+
+
+@pytest.mark.parametrize("vocab", [60, 5000, 70000])
+def test_extreme_temperatures_and_logits(vocab):
+    z, u = _logits(6, vocab, torch.float32)
+    for t in (1e-30, 1e-7, 1e-3, 30.0, 1e6, 1e30, 1e300):
+        for settings in (dict(temperature=t), dict(temperature=t, top_k=9), dict(temperature=t, top_p=0.7), dict(temperature=t, min_p=0.3, top_p=0.9)):
+            _check(z, u, **settings)
+    far = z.clone()
+    far[0] += 1e6
+    far[1] *= 1e30
+    far[2] = -3.4e38
+    far[2, :3] = -3.3e38
+    far[3] = torch.finfo(torch.float32).min
+    far[3, 5:] = float("-inf")
+    far[4] *= 1e-42                          # subnormal numbers
+    far[5] = 0.0
+    far[5, 7] = 1e-45
+    for t in (1e-40, 1.0, 1e37):
+        for settings in (dict(temperature=t), dict(temperature=t, top_k=4), dict(temperature=t, top_p=0.8), dict(temperature=t, min_p=0.5)):
+            _check(far, u, **settings)
+
+
+@pytest.mark.parametrize("offset", [0.0, 64.0, 3000.0, -500.0])
+def test_cuts_among_five_hundred(offset):
+    """Around the most logits that are sorted at once, with numbers far apart and equal ones on both sides."""
+    z, u = _logits(8, 30000, torch.float32)
+    z = z + offset
+    for dtype in (torch.float32, torch.bfloat16):
+        for k in (350, 500, 511, 512, 513, 600):
+            _check(z.to(dtype), u, top_k=k)
+            _check(z.to(dtype), u, top_k=k, top_p=0.97, temperature=2.0)
+        for p in (0.3, 0.45, 0.6):
+            _check(z.to(dtype), u, top_p=p)
+
+
 @pytest.mark.parametrize("vocab", [50, 3000, 40001])
 def test_equal_logits_rank_by_index(vocab):
     z = torch.zeros(6, vocab, device="cuda")
