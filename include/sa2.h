@@ -316,9 +316,10 @@ int sa2_step_attn(const sa2_qkvnorm_args *args, const sa2_append_set sets[4], vo
  * turns per position in units of 2^-64, so that the product with an integer position is exact modulo a turn.  positions (element
  * strides pos_batch, pos_seq, 0 allowed) is int64; null: row i of every sequence is at start + i.
  * x, dy: [b][n][heads][d], strides multiples of 16 bytes, 16-byte aligned; results [b][n][heads][d] contiguous.  gains: d
- * entries, 16-byte aligned.  d is 32, 64, 128 or 256, 2 * pairs <= d and a multiple of 16, b * n below 2^31.
+ * entries, 16-byte aligned.  d is 32, 64, 128 or 256, 2 * pairs <= d and a multiple of 16, b * n up to 2^30.
  * sa2_rotary_bwd reads x again and writes dx and the gains' gradients in gain_dtype, summed in a fixed order; `partial` is scratch of
  * sa2_rotary_partial_bytes().
+ * Results must not overlap inputs.
  */
 typedef struct sa2_rotary_side {
     const void *x, *dy;        /* dy: backward only */
@@ -374,7 +375,7 @@ int sa2_embed_bwd(const sa2_embed_args *args);
 size_t sa2_embed_workspace_bytes(int64_t rows, int32_t dim);
 
 /*
- * Distillation from a teacher's k largest logits of a row (k <= 1024):
+ * Distillation from a teacher's k largest logits of a row (k <= 1024, vocab <= 2^30):
  *   q = softmax(logits / T),  p = softmax(teacher / T) over the entries of the row
  *   loss[r] = T^2 sum_k p_k (log p_k - log q[index_k]),   dlogits_j = g T (q_j - sum of p_k over index_k == j)
  * Entries with an index outside [0, vocab) are not there; a row without entries (or with none above -inf) has loss and gradient
@@ -383,6 +384,7 @@ size_t sa2_embed_workspace_bytes(int64_t rows, int32_t dim);
  * entries, at least 1); either may be null.  The workspace (sa2_distill_workspace_bytes(), 256-byte aligned) keeps what sa2_distill_bwd needs
  * beside the logits; gout is the gradient of the total, or of every row (gout_rows != 0), null is 1.  sa2_distill_both is the forward and
  * the backward for gout = grad_scale, which reads the logits from memory once.
+ * dlogits must not overlap logits.
  */
 typedef enum sa2_reduction { SA2_SUM = 0, SA2_MEAN = 1 } sa2_reduction;
 typedef struct sa2_distill_args {
@@ -404,10 +406,10 @@ int sa2_distill_both(const sa2_distill_args *args);
 size_t sa2_distill_workspace_bytes(int64_t rows, int32_t k);
 
 /*
- * One token for each row of logits (fp32 or bf16, element stride 1): temperature, then the first top_k, then those before which less
+ * One token for each row of logits (fp32 or bf16, element stride 1, vocab <= 2^30): temperature, then the first top_k, then those before which less
  * than top_p of the remaining mass has come, then those at least min_p times as probable as the best; of what is kept, the first token by
  * index at which the running mass exceeds uniform[r] times the whole (the reference's sample() filters by top-k alone, train.py:104-109).
- * Equal logits rank by index.  temperature <= 0 takes the best token; top_k <= 0 or >= vocab, top_p >= 1 and min_p <= 0 are off.  Each may be
+ * Equal logits rank by index.  temperature <= 0 (or NaN) takes the best token; top_k <= 0 or >= vocab, top_p >= 1 and min_p <= 0 are off.  Each may be
  * given for every row (a device pointer) or once.  A row with a NaN or +inf, or of -inf alone, gets token -1 and log-probability NaN.
  * logprob (may be null): logarithm of the token's probability among what is kept.
  */

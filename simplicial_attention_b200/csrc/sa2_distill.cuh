@@ -61,7 +61,10 @@ __device__ __forceinline__ Factor factor(float t) {
     return f;
 }
 template <typename T> __device__ __forceinline__ float weight(float d, const Factor &f) {
-    if constexpr (sizeof(T) == 4) return ex2(d == -CUDART_INF_F ? d : fmaf(d, f.hi, d * f.lo));
+    if constexpr (sizeof(T) == 4) {
+        const float y = d * f.hi;                        // (far below, the second part may overflow)
+        return ex2(y < -200.f ? y : fmaf(d, f.hi, d * f.lo));
+    }
     else return ex2(d * f.hi);
 }
 
@@ -229,7 +232,8 @@ template <int G, typename T> __device__ __forceinline__ float2 joined(float2 all
     auto join = [&](float2 a, float2 b) {
         const float m = fmaxf(a.x, b.x);
         if (m == -CUDART_INF_F) return make_float2(m, a.y + b.y);
-        return make_float2(m, (a.x == -CUDART_INF_F ? 0.f : a.y * weight<T>(a.x - m, f)) + (b.x == -CUDART_INF_F ? 0.f : b.y * weight<T>(b.x - m, f)));
+        // (without a maximum the sum is 0, or NaN)
+        return make_float2(m, (a.x == -CUDART_INF_F ? a.y : a.y * weight<T>(a.x - m, f)) + (b.x == -CUDART_INF_F ? b.y : b.y * weight<T>(b.x - m, f)));
     };
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) all = join(all, make_float2(__shfl_xor_sync(0xffffffffu, all.x, o), __shfl_xor_sync(0xffffffffu, all.y, o)));
@@ -284,7 +288,7 @@ __global__ void __launch_bounds__(G == 32 ? 256 : G, G == 32 ? 4 : 1536 / G) fwd
 template <typename T, int G>
 __global__ void __launch_bounds__(G, 1024 / G) both_kernel(const __grid_constant__ Params P) {
     __shared__ float2 of_warp[G / 32];
-    __shared__ int counted;
+    __shared__ int counted[G / 32];
     extern __shared__ __align__(16) char shared[];
     const int64_t r = blockIdx.x;
     const T *row = reinterpret_cast<const T *>(P.z) + r * P.zs;
@@ -302,12 +306,11 @@ __global__ void __launch_bounds__(G, 1024 / G) both_kernel(const __grid_constant
         }
     });
     const bool there = P.there[r];
-    if (P.mean && threadIdx.x < 32) {                    // rows that count
+    if (P.mean) {                                        // rows that count
         int rows = 0;
-        for (int64_t x = threadIdx.x; x < (P.rows + TEACHER_ROWS - 1) / TEACHER_ROWS; x += 32) rows += P.counts[x];
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) rows += __shfl_xor_sync(0xffffffffu, rows, o);
-        if (threadIdx.x == 0) counted = rows;
+        for (int64_t x = threadIdx.x; x < (P.rows + TEACHER_ROWS - 1) / TEACHER_ROWS; x += G) rows += P.counts[x];
+        rows = __reduce_add_sync(0xffffffffu, rows);
+        if (threadIdx.x % 32 == 0) counted[threadIdx.x / 32] = rows;
     }
     for (int k = threadIdx.x; k < P.k; k += G) {
         place[k] = P.place[r * P.k + k];
@@ -315,7 +318,8 @@ __global__ void __launch_bounds__(G, 1024 / G) both_kernel(const __grid_constant
     }
     const float2 all = joined<G, T>(make_float2(run.m, run.s), of_warp, f);
     const float ref = all.x == -CUDART_INF_F ? 0.f : all.x, s = all.y;
-    const int rows = P.mean ? counted : 1;
+    int rows = P.mean ? 0 : 1;
+    for (int w = 0; P.mean && w < G / 32; ++w) rows += counted[w];
     const float coef = (float)(1. / (double)max(rows, 1)) * P.times * P.t, inv = 1.f / s;
     const bool together = ((reinterpret_cast<uintptr_t>(row) ^ reinterpret_cast<uintptr_t>(grad)) & 15) == 0;
     for_row<G, T, 8>(row, P.vocab, [&](int x, int count, float (&v)[8]) {

@@ -46,7 +46,7 @@ int rotary_check(const sa2_rotary_args *a, bool backward) {
     if (!known(a->dtype) || !known(a->gain_dtype)) return SA2_ERR_UNSUPPORTED;
     if (a->d != 32 && a->d != 64 && a->d != 128 && a->d != 256) return SA2_ERR_UNSUPPORTED;
     if (a->pairs <= 0 || a->pairs % 8 || 2 * a->pairs > a->d) return SA2_ERR_UNSUPPORTED;
-    if ((int64_t)a->b * a->n > INT32_MAX || (int64_t)a->q.heads + a->k.heads > 4096) return SA2_ERR_UNSUPPORTED;
+    if ((int64_t)a->b * a->n > 1 << 30 || (int64_t)a->q.heads + a->k.heads > 4096) return SA2_ERR_UNSUPPORTED;
     for (const sa2_rotary_side *s : {&a->q, &a->k}) {
         if (!s->x || !s->y || !s->gain || !aligned16(s->x) || !aligned16(s->y) || !aligned16(s->gain) || !rotary_strides_ok(s->sx, a->dtype)) return SA2_ERR_INVALID;
         if (backward && (!s->dy || !s->dgain || !aligned16(s->dy) || !rotary_strides_ok(s->sdy, a->dtype))) return SA2_ERR_INVALID;
@@ -167,9 +167,10 @@ int distill_check(const sa2_distill_args *a, bool forward, bool backward) {
     if (!a || !a->logits || a->rows <= 0 || a->vocab <= 0 || a->k <= 0) return SA2_ERR_INVALID;
     if (forward && (!a->teacher || !a->index || (!a->row_loss && !a->total))) return SA2_ERR_INVALID;
     if (backward && !a->dlogits) return SA2_ERR_INVALID;
-    if (!known(a->dtype) || !known(a->teacher_dtype) || a->k > sa2::distill::MAX_K || a->rows > INT32_MAX) return SA2_ERR_UNSUPPORTED;
+    if (!known(a->dtype) || !known(a->teacher_dtype) || a->k > sa2::distill::MAX_K || a->rows > INT32_MAX || a->vocab > 1 << 30) return SA2_ERR_UNSUPPORTED;
     if (a->reduction != SA2_SUM && a->reduction != SA2_MEAN) return SA2_ERR_UNSUPPORTED;
-    if (!(a->temperature > 0.f) || a->temperature * 0.f != 0.f) return SA2_ERR_INVALID;
+    // (log2(e) / T is an fp32 number in the kernels)
+    if (!(a->temperature > 4.5e-39f) || a->temperature * 0.f != 0.f) return SA2_ERR_INVALID;
     const uintptr_t unit = size_of(a->dtype) - 1;
     if ((reinterpret_cast<uintptr_t>(a->logits) & unit) || (backward && (reinterpret_cast<uintptr_t>(a->dlogits) & unit))) return SA2_ERR_INVALID;
     if (!a->workspace || (reinterpret_cast<uintptr_t>(a->workspace) & 255u) || a->workspace_bytes < sa2_distill_workspace_bytes(a->rows, a->k))
@@ -304,7 +305,7 @@ int sa2_distill_both(const sa2_distill_args *a) {
 int sa2_sample(const sa2_sample_args *a) {
     Range range("sa2_sample");
     if (!a || !a->logits || !a->uniform || !a->token || a->rows <= 0 || a->vocab <= 0) return SA2_ERR_INVALID;
-    if (!known(a->dtype)) return SA2_ERR_UNSUPPORTED;
+    if (!known(a->dtype) || a->vocab > 1 << 30) return SA2_ERR_UNSUPPORTED;
     if (reinterpret_cast<uintptr_t>(a->logits) & (size_of(a->dtype) - 1)) return SA2_ERR_INVALID;
     namespace sm = sa2::sample;
     sm::Params P{};

@@ -578,7 +578,7 @@ pybind11::object qk_norm_rotary(const Tensor &q, const Tensor &k, const Tensor &
         const bool whole = p.dim() == 2 && (p.size(0) == q.size(0) || p.size(0) == 1);
         if (p.scalar_type() != at::kLong || !(p.dim() == 1 || whole) || p.size(-1) != q.size(1)) return pybind11::none();
     }
-    if (q.size(0) * q.size(1) > INT32_MAX) return pybind11::none();
+    if (q.size(0) * q.size(1) > 1 << 30) return pybind11::none();
     const auto r = Rotary::apply(q, k, gq, gk, freqs, positions, start, eps, interleaved);
     return pybind11::make_tuple(r[0], r[1]);
 }
@@ -619,7 +619,11 @@ struct Embed : torch::autograd::Function<Embed> {
         const bool want_w = ctx->needs_input_grad(1), want_p = position_rows >= 0 && ctx->needs_input_grad(2);
         Tensor dw, dp;
         if (at::GradMode::is_enabled()) {                // a backward of this backward: in torch's operators
-            if (want_w) dw = at::embedding_dense_backward(grads[0] * scale, tokens.to(at::kLong), vocab, padding, false);
+            if (want_w) {
+                // (tokens outside of the table have no gradient there either)
+                const Tensor t = tokens.to(at::kLong), outside = at::logical_or(t.lt(0), t.ge(vocab));
+                dw = at::embedding_dense_backward((grads[0] * scale).masked_fill(outside.unsqueeze(-1), 0), t.masked_fill(outside, 0), vocab, padding, false);
+            }
             if (want_p) dp = at::constant_pad_nd(grads[0].reshape({-1, n, dim}).sum(0), {0, 0, start, position_rows - start - n});
         } else {
             const Tensor dout = grads[0].contiguous();
@@ -722,7 +726,7 @@ bool distill_ok(const Tensor &logits, const Tensor &teacher, const Tensor &index
         if (!plain(*t, logits.device()) || t->dim() < 1 || t->dim() != logits.dim() || t->sizes().slice(0, t->dim() - 1) != logits.sizes().slice(0, logits.dim() - 1)) return false;
     if (dtype_of(logits) < 0 || dtype_of(teacher) < 0 || (index.scalar_type() != at::kLong && index.scalar_type() != at::kInt)) return false;
     const int64_t vocab = logits.size(-1), k = teacher.size(-1);
-    return vocab > 0 && vocab <= INT32_MAX && k > 0 && k <= 1024 && index.size(-1) == k && logits.numel() / vocab <= INT32_MAX;
+    return vocab > 0 && vocab <= 1 << 30 && k > 0 && k <= 1024 && index.size(-1) == k && logits.numel() / vocab <= INT32_MAX;
 }
 pybind11::object distill(const Tensor &logits, const Tensor &teacher, const Tensor &index, double t, int64_t reduction) {
     if (!distill_ok(logits, teacher, index)) return pybind11::none();
@@ -744,7 +748,7 @@ pybind11::object sample(const Tensor &logits, const Tensor &uniform, const std::
                         int64_t top_k_all, const std::optional<Tensor> &top_p, double top_p_all, const std::optional<Tensor> &min_p, double min_p_all, bool logprobs) {
     if (tracing() || !plain(logits, logits.device()) || !plain(uniform, logits.device()) || logits.dim() < 1 || dtype_of(logits) < 0) return pybind11::none();
     const auto shape = logits.sizes().slice(0, logits.dim() - 1);
-    if (uniform.sizes() != shape || (uniform.scalar_type() != at::kFloat && uniform.scalar_type() != at::kDouble) || logits.size(-1) == 0 || logits.size(-1) > INT32_MAX) return pybind11::none();
+    if (uniform.sizes() != shape || (uniform.scalar_type() != at::kFloat && uniform.scalar_type() != at::kDouble) || logits.size(-1) == 0 || logits.size(-1) > 1 << 30) return pybind11::none();
     const int64_t vocab = logits.size(-1), rows = logits.numel() / vocab;
     for (const auto *t : {&temperature, &top_p, &min_p})
         if (*t && (!plain(**t, logits.device()) || (*t)->scalar_type() != at::kFloat || (*t)->sizes() != shape || !(*t)->is_contiguous())) return pybind11::none();

@@ -22,13 +22,13 @@ def _refuse(logits, teacher_logits, teacher_index, temperature, reduction, reduc
         raise ValueError("logits must be float32 or bfloat16, the teacher's indices int64 or int32")
     if logits.dim() < 1 or teacher_logits.shape != teacher_index.shape or teacher_logits.shape[:-1] != logits.shape[:-1]:
         raise ValueError("expected logits of (..., vocab) and the teacher's logits and indices of (..., k)")
-    if logits.shape[-1] == 0 or not 1 <= teacher_logits.shape[-1] <= 1024:
-        raise ValueError("the vocabulary must not be empty, and the teacher has 1 to 1024 entries")
+    if not 1 <= logits.shape[-1] <= 2 ** 30 or not 1 <= teacher_logits.shape[-1] <= 1024:
+        raise ValueError("the vocabulary must have 1 to 2^30 entries, and the teacher 1 to 1024")
     raise RuntimeError("distillation takes plain tensors of one device, outside of tracing and transforms")
 
 
 def _check(temperature, reduction, reductions):
-    if not (math.isfinite(temperature) and temperature > 0):
+    if not 5e-39 <= temperature <= 3e38:                 # fp32 in the kernels, and its inverse
         raise ValueError(f"temperature must be positive and finite, not {temperature}")
     if reduction not in reductions:
         raise ValueError(f"reduction must be one of {', '.join(reductions)}, not {reduction!r}")

@@ -20,8 +20,14 @@ def token_embedding(tokens: Tensor, weight: Tensor, pos_weight: Tensor | None = 
     ``tokens``: int64 or int32, ``(..., n)``; ``weight``: ``(vocab, dim)``, fp32 or bf16; ``pos_weight``: ``(positions, dim)`` of the same
     dtype, of which the last dimension of ``tokens`` takes rows ``start`` on.  A token outside ``[0, vocab)`` reads nothing: its row is
     NaN, and it has no gradient.  The gradients are dense; sums run over the sorted tokens in fp32 in one order, so that they are the
-    same bits from run to run.  The row ``padding_idx`` of the table gets no gradient."""
-    out = _lib.ext().embed(tokens, weight, pos_weight, float(scale), int(start), -1 if padding_idx is None else int(padding_idx))
+    same bits from run to run.  The row ``padding_idx`` of the table (negative: from its end, as in ``nn.Embedding``)
+    gets no gradient."""
+    padding = -1 if padding_idx is None else int(padding_idx)
+    if padding_idx is not None and weight.dim() == 2:
+        if not -weight.shape[0] <= padding < weight.shape[0]:
+            raise ValueError(f"padding_idx {padding} is outside of the table")
+        padding %= weight.shape[0]
+    out = _lib.ext().embed(tokens, weight, pos_weight, float(scale), int(start), padding)
     if out is not None:
         return out
     tensors = [t for t in (tokens, weight, pos_weight) if t is not None]

@@ -43,7 +43,7 @@ def qk_norm_rotary(q: Tensor, k: Tensor, q_weight: Tensor, k_weight: Tensor, fre
     channels ``(i, i + rotated / 2)``, or ``(2 i, 2 i + 1)`` if ``interleaved``.  Row ``i`` is at position ``start + i``, or at
     ``positions`` - int64, ``(n,)`` or ``(b, n)``, any value: the angle is exact modulo a turn.  ``eps`` defaults to the dtype's machine epsilon.
     Results are ``(b, n, heads, d)``, contiguous, in the dtype of ``q`` and ``k``; everything in between is fp32."""
-    eps = torch.finfo(q.dtype).eps if eps is None else float(eps)
+    eps = float(eps) if eps is not None else torch.finfo(q.dtype).eps if q.dtype in _DTYPES else 0.0
     res = _lib.ext().qk_norm_rotary(q, k, q_weight, k_weight, freqs, positions, int(start), eps, bool(interleaved))
     if res is not None:
         return res
@@ -63,7 +63,7 @@ def qk_norm_rotary(q: Tensor, k: Tensor, q_weight: Tensor, k_weight: Tensor, fre
     if positions is not None and (positions.dtype != torch.int64 or positions.dim() not in (1, 2) or positions.shape[-1] != q.shape[1]
                                   or (positions.dim() == 2 and positions.shape[0] not in (1, q.shape[0]))):
         raise ValueError("positions must be int64 of (seq,) or (batch, seq)")
-    raise RuntimeError("qk_norm_rotary takes plain tensors of one device (below 2^31 rows, 4096 heads), outside of tracing and transforms")
+    raise RuntimeError("qk_norm_rotary takes plain tensors of one device (up to 2^30 rows, 4096 heads), outside of tracing and transforms")
 
 
 def _plain(q, k, q_weight, k_weight, freqs, start, eps, interleaved=False):

@@ -56,8 +56,8 @@ def sample_tokens(logits: Tensor, uniform: Tensor, *, temperature=1.0, top_k=Non
         if logits.dtype not in _DTYPES or uniform.dtype not in (torch.float32, torch.float64):
             raise ValueError("logits must be float32 or bfloat16, uniform float32 or float64")
         rows = logits.shape[:-1]
-        if logits.dim() < 1 or logits.shape[-1] == 0 or uniform.shape != rows:
-            raise ValueError("expected logits of (..., vocab) and a uniform number for each row")
+        if logits.dim() < 1 or not 1 <= logits.shape[-1] <= 2 ** 30 or uniform.shape != rows:
+            raise ValueError("expected logits of (..., vocab), vocab up to 2^30, and a uniform number for each row")
         res = call(*(v if isinstance(v, Tensor) else None for v in (
             _setting(temperature, "temperature", rows, logits, torch.float32), _setting(top_k, "top_k", rows, logits, torch.int64),
             _setting(top_p, "top_p", rows, logits, torch.float32), _setting(min_p, "min_p", rows, logits, torch.float32))))

@@ -156,6 +156,50 @@ def test_strided_rows_and_shapes(vocab, dtype):
     assert torch.equal(sa.distillation_loss(three[1, 2], t[5], i[5], reduction="none"), a[1, 2])
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("vocab,first,count", [(5, 0, 1), (5, 4, 1), (50, 8, 8), (4097, 800, 8), (4097, 0, 4097)])
+def test_nan_anywhere_shows(vocab, first, count, dtype):
+    z, t, i = _inputs(3, vocab, 4, dtype)
+    clean = sa.distillation_loss(z, t, i, reduction="none")
+    z[1, first:first + count] = float("nan")
+    leaf = z.clone().requires_grad_()
+    loss = sa.distillation_loss(leaf, t, i, reduction="none")
+    loss.sum().backward()
+    assert loss[1].isnan() and torch.equal(loss[::2], clean[::2])
+    assert leaf.grad[1].isnan().all() and not leaf.grad[::2].isnan().any()
+    total, grad = sa.distillation_loss_and_grad(z, t, i)
+    assert total.isnan() and grad[1].isnan().all() and not grad[::2].isnan().any()
+
+
+@pytest.mark.parametrize("temperature", [1e-30, 1e-8, 1e38])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("vocab", [300, 4099])
+def test_lowest_values_and_temperatures_far_from_one(vocab, dtype, temperature):
+    z = torch.full((2, vocab), torch.finfo(dtype).min, dtype=dtype, device="cuda")
+    z[:, 7], z[0, 9] = 2.0, 2.0
+    t, i = torch.tensor([[1.0, 1.0], [3.0, 3.0]], device="cuda"), torch.tensor([[7, 9], [7, 7]], device="cuda")
+    _, dz, *_ = _oracle(z, t, i, float(torch.tensor(temperature, dtype=torch.float32)))
+    leaf = z.requires_grad_()
+    both = sa.distillation_loss_and_grad(z.detach(), t, i, reduction="sum", temperature=temperature)[1]
+    grad = torch.autograd.grad(sa.distillation_loss(leaf, t, i, reduction="sum", temperature=temperature), leaf)[0]
+    # exponents of the lowest value at T = 1e38 are off by their rounding, 2^-23 of 4.9; the sum of a row and its inverse as above
+    bound = temperature * ((vocab / 32 + 100) * U + 1.0 / vocab * _half_step(z)) + dz.abs() * _half_step(z) + 2.0 ** -133
+    assert ((grad.double() - dz).abs() <= bound).all() and ((both.double() - dz).abs() <= bound).all()
+
+
+def test_mean_over_many_rows():
+    z, t, i = _inputs(20000, 2100, 2, torch.bfloat16)
+    i[::3] = -1
+    loss, grad = sa.distillation_loss_and_grad(z, t, i)
+    rows = sa.distillation_loss(z, t, i, reduction="none").double()
+    counted = 20000 - len(range(0, 20000, 3))
+    want = rows.sum() / counted
+    assert (loss.double() - want).abs() <= want.abs() * 2 * U
+    leaf = z.requires_grad_()
+    assert torch.equal(torch.autograd.grad(sa.distillation_loss(leaf, t, i), leaf)[0], grad)
+    assert (grad[::3] == 0).all() and (grad[1::3] != 0).any()
+
+
 def test_nothing():
     z, t, i = torch.zeros(0, 7, device="cuda"), torch.zeros(0, 2, device="cuda"), torch.zeros(0, 2, dtype=torch.long, device="cuda")
     leaf = z.requires_grad_()

@@ -160,6 +160,28 @@ def test_backward_of_the_backward():
         want = second
 
 
+def test_backward_of_the_backward_with_tokens_outside():
+    tokens, weight, _, dout = _case((2, 30), 11, 16, torch.float32)
+    tokens[0, :9] = -1
+    tokens[1, 3] = 11
+    tokens[1, 5:8] = 4
+    dout.requires_grad_()
+    out = sa.token_embedding(tokens, weight, padding_idx=4)
+    grad = torch.autograd.grad(out, weight, dout, create_graph=True)[0]
+    second = torch.autograd.grad(grad.square().sum(), dout)[0]
+    counts = (tokens >= 0) & (tokens < 11) & (tokens != 4)
+    assert (second[~counts] == 0).all() and (second[counts] != 0).any()
+    plain = torch.autograd.grad(sa.token_embedding(tokens, weight, padding_idx=4), weight, dout)[0]
+    assert (grad - plain).abs().max() <= 60 * U * plain.abs().max() * 4
+
+
+def test_padding_from_the_end():
+    tokens, weight, _, dout = _case((2, 30), 11, 16, torch.float32)
+    tokens[0, :5] = 10
+    got = [torch.autograd.grad(sa.token_embedding(tokens, weight, padding_idx=x), weight, dout)[0] for x in (10, -1)]
+    assert torch.equal(*got) and (got[0][10] == 0).all()
+
+
 def test_captured():
     tokens, weight, pos, dout = _case((4, 600), 100, 64, torch.bfloat16, 600)
     weight, pos = weight.detach(), pos.detach()

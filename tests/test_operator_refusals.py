@@ -36,6 +36,9 @@ def test_embedding():
                            ((ids, _cuda(8)), {}, "dim"), ((ids, _cuda(0, 8)), {}, "dim"), ((ids, w, p), dict(start=3), "positions"), ((ids, w, p), dict(start=-1), "positions")]:
         with pytest.raises(ValueError, match=what):
             sa.token_embedding(*args, **kw)
+    for padding in (9, -10):
+        with pytest.raises(ValueError, match="padding_idx"):
+            sa.token_embedding(ids, w, padding_idx=padding)
     with pytest.raises(RuntimeError, match="plain tensors"):
         sa.token_embedding(ids, w, p)                    # no values to read
 
@@ -64,7 +67,7 @@ def test_rotary():
 @pytest.mark.parametrize("call", [sa.distillation_loss, sa.distillation_loss_and_grad])
 def test_distillation(call):
     z, t, i = _cuda(4, 50), _cuda(4, 3), _cuda(4, 3, dtype=torch.long)
-    for temperature in (0.0, -1.0, math.inf, math.nan):
+    for temperature in (0.0, -1.0, 1e-40, 1e39, math.inf, math.nan):
         with pytest.raises(ValueError, match="temperature"):
             call(z, t, i, temperature=temperature)
     with pytest.raises(ValueError, match="reduction"):
@@ -154,12 +157,12 @@ def test_c_calls_of_the_embedding():
 
 def test_c_calls_of_sampling_and_distillation():
     lib = _lib.lib()
-    for kw, status in [(dict(logits=0), 1), (dict(uniform=0), 1), (dict(token=0), 1), (dict(rows=0), 1), (dict(vocab=-1), 1), (dict(dtype=3), 2), (dict(logits=A + 2), 1)]:
+    for kw, status in [(dict(logits=0), 1), (dict(uniform=0), 1), (dict(token=0), 1), (dict(rows=0), 1), (dict(vocab=-1), 1), (dict(vocab=(1 << 30) + 1), 2), (dict(dtype=3), 2), (dict(logits=A + 2), 1)]:
         assert lib.sa2_sample(C.byref(SampleArgs(**{**dict(logits=A, uniform=A, token=A, rows=2, vocab=5), **kw}))) == status
     assert lib.sa2_sample(None) == 1
     good = dict(logits=A, teacher=A, index=A, row_loss=A, total=A, dlogits=A, workspace=A, workspace_bytes=1 << 20, rows=3, vocab=9, k=2, temperature=1.0)
     for kw, status in [(dict(logits=0), 1), (dict(rows=0), 1), (dict(workspace=0), 3), (dict(workspace=A + 16), 3), (dict(workspace_bytes=300), 3), (dict(vocab=0), 1), (dict(k=0), 1),
-                       (dict(k=1025), 2), (dict(dtype=5), 2), (dict(teacher_dtype=5), 2), (dict(reduction=4), 2), (dict(temperature=0.0), 1), (dict(temperature=math.inf), 1),
+                       (dict(k=1025), 2), (dict(vocab=(1 << 30) + 1), 2), (dict(dtype=5), 2), (dict(teacher_dtype=5), 2), (dict(reduction=4), 2), (dict(temperature=0.0), 1), (dict(temperature=1e-40), 1), (dict(temperature=math.inf), 1),
                        (dict(temperature=math.nan), 1), (dict(logits=A + 2), 1)]:
         a = C.byref(DistillArgs(**{**good, **kw}))
         assert lib.sa2_distill_fwd(a) == status and lib.sa2_distill_bwd(a) == status and lib.sa2_distill_both(a) == status
