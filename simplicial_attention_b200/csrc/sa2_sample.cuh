@@ -437,8 +437,8 @@ __device__ Cut find_cut(const Row<T, RESIDENT> &R, const View &V, Shared<N> &S, 
     }
 }
 
-// The stretches [S.first_bin, S.last_bin] of the coarse histogram that hold the cut, for a wanted count or mass between `least` and `most`.  A stretch's logits are less than (bin + 1) width and at least
-// bin width below the maximum, but for the roundings that the margins cover.
+// The stretches [S.first_bin, S.last_bin] of the coarse histogram that hold the cut, for a wanted count or mass between `least` and `most`.  A
+// stretch's logits are less than (bin + 1) width and at least bin width below the maximum, but for the roundings that the margins cover.
 template <int N> __device__ __forceinline__ void bracket(Shared<N> &S, double width, double inv_t, bool by_mass, double least, double most) {
     const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
     const double c = (double)S.total[t];
@@ -471,6 +471,7 @@ __global__ void __launch_bounds__(N, 1024 / N) kernel(const __grid_constant__ Pa
     const int begin = min(P.vocab, rank * P.slice), slice = min(P.slice, P.vocab - begin);
     const T *src = reinterpret_cast<const T *>(P.z) + row * P.zs + begin;
     T *own = reinterpret_cast<T *>(smem + sizeof(Shared<N>));
+    if (ctas > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
     Row<T, RESIDENT> R;
     R.z = RESIDENT ? own : src;
     R.ring = own + warp * RING * 128;
@@ -529,6 +530,8 @@ __global__ void __launch_bounds__(N, 1024 / N) kernel(const __grid_constant__ Pa
     __syncthreads();
     for (int w = 0; w < WARPS<N>; ++w) best = fmaxf(best, (float)S.warp_low[w]);
     if (ctas > 1) {
+        // (all CTAs of the cluster run: their shared memory may be written)
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
         if (threadIdx.x < ctas) of_cta(S, ctas, threadIdx.x).max_of[rank] = best;
         row_sync(ctas);
         for (int r = 0; r < ctas; ++r) best = fmaxf(best, S.max_of[r]);
