@@ -186,26 +186,30 @@ sa2::distill::Params distill_params(const sa2_distill_args *a) {
     P.times = a->grad_scale;
     P.rows = a->rows; P.zs = a->logits_stride; P.ts = a->teacher_stride; P.is = a->index_stride; P.ds = a->dlogits_stride;
     P.vocab = a->vocab; P.k = a->k; P.index64 = a->index64; P.teacher_bf16 = a->teacher_dtype == SA2_BF16; P.t = a->temperature;
+    const double c = 1.4426950408889634 / (double)a->temperature;
+    P.hi = (float)c; P.lo = (float)(c - (double)P.hi);
     sa2::distill::carve(P, a->workspace);
     if (a->row_loss) P.row_loss = a->row_loss;
     return P;
 }
 
-// a warp a row up to this vocabulary
-constexpr int WARP_VOCAB = 2048;
+// Threads of a row, by its bytes: what a CTA does once costs every warp alike, and more rows at a time wait for one another.  Loss and gradient at
+// once, with 128, 256 and 512 threads: 136, 187 and 305 us (16384 rows of 4096 bf16 logits), 162, 170 and 218 (8192 of 10000 fp32), 275, 240
+// and 276 (8192 of 32000 bf16), 285, 256 and 234 (4095 of 32000 fp32), 563, 520 and 476 (4096 of 128000 bf16).  Short rows have a warp.
+template <typename T> inline int distill_threads(int vocab) {
+    const int64_t bytes = (int64_t)vocab * sizeof(T);
+    return vocab <= 2048 ? 32 : bytes <= 48 * 1024 ? 128 : bytes <= 112 * 1024 ? 256 : 512;
+}
 
 template <typename T> int distill_bwd(const sa2_distill_args *a) {
     sa2::distill::Params P = distill_params(a);
     if (!P.mean || a->gout_rows) P.scale = nullptr;
     cudaStream_t st = stream_of(a->stream);
-    const size_t entries = (size_t)a->k * 8;
-    if (a->vocab <= WARP_VOCAB) {
-        const auto kernel = sa2::distill::bwd_kernel<T, 32>;
-        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 8 * sa2::distill::MAX_K * 8) != cudaSuccess) return SA2_ERR_CUDA;
-        kernel<<<(unsigned)((a->rows + 7) / 8), 256, 8 * entries, st>>>(P);
-    } else {
-        sa2::distill::bwd_kernel<T, 512><<<(unsigned)a->rows, 512, entries, st>>>(P);
-    }
+    const int g = distill_threads<T>(a->vocab);
+    if (g == 32) sa2::distill::bwd_kernel<T, 32><<<(unsigned)((a->rows + 7) / 8), 256, 0, st>>>(P);
+    else if (g == 128) sa2::distill::bwd_kernel<T, 128><<<(unsigned)a->rows, 128, 0, st>>>(P);
+    else if (g == 256) sa2::distill::bwd_kernel<T, 256><<<(unsigned)a->rows, 256, 0, st>>>(P);
+    else sa2::distill::bwd_kernel<T, 512><<<(unsigned)a->rows, 512, 0, st>>>(P);
     return launch_status();
 }
 
@@ -214,12 +218,18 @@ template <typename T> int distill_fwd(const sa2_distill_args *a, bool grad) {
     const sa2::distill::Params P = distill_params(a);
     cudaStream_t st = stream_of(a->stream);
     using namespace sa2::distill;
-    teacher_kernel<<<(unsigned)teacher_blocks(a->rows), 32 * TEACHER_ROWS, 0, st>>>(P);
+    const int warps = teacher_warps(a->k);
+    const size_t smem = (size_t)warps * teacher_words(a->k) * 4;
+    if (cudaFuncSetAttribute(teacher_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return SA2_ERR_CUDA;
+    teacher_kernel<<<(unsigned)teacher_blocks(a->rows), 32 * warps, smem, st>>>(P);
     if (int e = launch_status()) return e;
-    const bool both = grad && a->vocab > WARP_VOCAB;
-    if (both) both_kernel<T, 512><<<(unsigned)a->rows, 512, (size_t)a->k * 8, st>>>(P);
-    else if (a->vocab <= WARP_VOCAB) fwd_kernel<T, 32><<<(unsigned)((a->rows + 7) / 8), 256, 0, st>>>(P);
-    else fwd_kernel<T, 512><<<(unsigned)a->rows, 512, 0, st>>>(P);
+    const int g = distill_threads<T>(a->vocab);
+    const bool both = grad && g > 32;
+    const unsigned rows = (unsigned)a->rows;
+    if (g == 32) fwd_kernel<T, 32><<<(rows + 7) / 8, 256, 0, st>>>(P);
+    else if (g == 128) both ? both_kernel<T, 128><<<rows, 128, 0, st>>>(P) : fwd_kernel<T, 128><<<rows, 128, 0, st>>>(P);
+    else if (g == 256) both ? both_kernel<T, 256><<<rows, 256, 0, st>>>(P) : fwd_kernel<T, 256><<<rows, 256, 0, st>>>(P);
+    else both ? both_kernel<T, 512><<<rows, 512, 0, st>>>(P) : fwd_kernel<T, 512><<<rows, 512, 0, st>>>(P);
     if (int e = launch_status()) return e;
     if (a->total) {
         total_kernel<<<1, 1024, 0, st>>>(P.row_loss, P.counts, a->rows, P.mean, a->total, P.scale);
