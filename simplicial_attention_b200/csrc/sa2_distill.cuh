@@ -118,14 +118,15 @@ template <int G> struct Group {
 // Calls f(first element, number, values) for all of a row: pieces of eight from the first 16-byte boundary on, U at a time (half as many of fp32),
 // single elements around them.  AHEAD: half of the U are loaded while the other half is used (for loss and gradient at once 105 instead of
 // 124 us at 8192 rows of 10000 bf16 logits, 187 instead of 204 at 4096 of 50257; the forward alone, with fewer registers, 239 instead of 224 at
-// 4096 of 128000).
-template <int G, typename T, int U, bool AHEAD, typename F> __device__ __forceinline__ void for_row(const T *row, int vocab, F f) {
+// 4096 of 128000).  BACK: from the last piece to the first.
+template <int G, typename T, int U, bool AHEAD, bool BACK = false, typename F> __device__ __forceinline__ void for_row(const T *row, int vocab, F f) {
     constexpr int V = (sizeof(T) == 2 ? U : U / 2) / (AHEAD ? 2 : 1);
     const int rank = Group<G>::rank();
     int head = (int)((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / (int)sizeof(T);
     if (head > vocab) head = vocab;
     const int pieces = (vocab - head) / 8;
     const T *from = row + head;
+    auto piece = [&](int x) { return BACK ? pieces - 1 - x : x; };
     auto one = [&](int x) {
         float v[8] = {(float)row[x]};
         f(x, 1, v);
@@ -133,7 +134,7 @@ template <int G, typename T, int U, bool AHEAD, typename F> __device__ __forcein
     auto load = [&](Packed<T> (&t)[V], int x0) {
 #pragma unroll
         for (int u = 0; u < V; ++u)
-            if (x0 + u * G < pieces) t[u].load(from + (x0 + u * G) * 8);
+            if (x0 + u * G < pieces) t[u].load(from + piece(x0 + u * G) * 8);
     };
     auto use = [&](const Packed<T> (&t)[V], int x0) {
 #pragma unroll
@@ -141,7 +142,7 @@ template <int G, typename T, int U, bool AHEAD, typename F> __device__ __forcein
             if (x0 + u * G < pieces) {
                 float v[8];
                 t[u].get(v);
-                f(head + (x0 + u * G) * 8, 8, v);
+                f(head + piece(x0 + u * G) * 8, 8, v);
             }
     };
     for (int x = rank; x < head; x += G) one(x);
@@ -352,7 +353,7 @@ template <int G, typename T, int U, bool ONCE> __device__ __forceinline__ void g
         return;
     }
     if (sizeof(T) == 2) g *= ex2(ref.off);
-    for_row<G, T, U, true>(row, vocab, [&](int x, int count, float (&v)[8]) {
+    for_row<G, T, U, true, ONCE>(row, vocab, [&](int x, int count, float (&v)[8]) {
 #pragma unroll
         for (int z = 0; z < 8; ++z) v[z] = g * ref.template weight_of<sizeof(T) == 2>(v[z], f);
         if (count != 8) {
@@ -404,11 +405,12 @@ __global__ void __launch_bounds__(G == 32 ? 256 : G, G == 32 ? 4 : 1536 / G) fwd
     }
 }
 
-// Loss and gradient: a CTA reads its row twice, the second time from L2, where the rows of all CTAs together have room (two CTAs of 512 threads an
-// SM, 76 MB at 128000 bf16 logits); gradients are stored so that they leave L2 first.  4096 such rows: 450 us, 325 at the rate of a copy.
-// A fifth of the second reads still miss L2, and ex2, twice a logit, would take 230 us alone.  Slower: rows in the shared memory of
-// clusters of four and eight CTAs, read once (576 us; 1080 with the next row on its way meanwhile: waits for the cluster, and for its places in one
-// GPC); two CTAs a row (524); 104 KB of each row kept in shared memory by the threads that read it (519, with 484 without at that time).
+// Loss and gradient: a CTA reads its row twice, the second time from the end to the beginning and from L2, which holds most of the rows of all
+// CTAs together (two CTAs of 512 threads an SM, 76 MB at 128000 bf16 logits; in one direction every second read missed it); gradients are stored
+// so that they leave L2 first.  4096 such rows: 420 us (450 in one direction), 325 at the rate of a copy; ex2, twice a logit, would take 230 us
+// alone.  Slower: rows in the shared memory of clusters of four and eight CTAs, read once (576 us; 1080 with the next row on its way
+// meanwhile: waits for the cluster, and for its places in one GPC); two CTAs a row (524); 104 KB of each row kept in shared memory by the threads
+// that read it (519, with 484 without at that time).
 template <typename T, int G>
 __global__ void __launch_bounds__(G, 1024 / G) both_kernel(const __grid_constant__ Params P) {
     __shared__ float2 of_warp[G / 32];
