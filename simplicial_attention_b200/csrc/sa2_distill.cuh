@@ -407,7 +407,7 @@ __global__ void __launch_bounds__(G == 32 ? 256 : G, G == 32 ? 4 : 1536 / G) fwd
 
 // Loss and gradient: a CTA reads its row twice, the second time from the end to the beginning and from L2, which holds most of the rows of all
 // CTAs together (two CTAs of 512 threads an SM, 76 MB at 128000 bf16 logits; in one direction every second read missed it); gradients are stored
-// so that they leave L2 first.  4096 such rows: 420 us (450 in one direction), 325 at the rate of a copy; ex2, twice a logit, would take 230 us
+// so that they leave L2 first.  4096 such rows: 430 us (450 in one direction), 325 at the rate of a copy; ex2, twice a logit, would take 230 us
 // alone.  Slower: rows in the shared memory of clusters of four and eight CTAs, read once (576 us; 1080 with the next row on its way
 // meanwhile: waits for the cluster, and for its places in one GPC); two CTAs a row (524); 104 KB of each row kept in shared memory by the threads
 // that read it (519, with 484 without at that time).

@@ -4,13 +4,15 @@
 //   dW[t] = scale * sum of dout[b, i] over all (b, i) with token[b, i] == t,   dP[start + i] = sum over b of dout[b, i]
 // A token outside [0, vocab) reads nothing: its row of out is NaN, and it has no gradient; nor has the padding token.
 //
-// Forward: HBM-bound copies of rows, 16 bytes a lane and access, the pieces of four bf16 or two fp32 rows in flight.
+// Forward: HBM-bound copies of rows, 16 bytes a lane and access, the pieces of four bf16 or two fp32 rows in flight (16384 rows of 2048 bf16
+// channels 20 us, 6.7 TB/s with rows that L2 holds).
 //
 // Backward, three launches.  (1) One cluster sorts the tokens with their places, stably, while the other CTAs of the launch write the zeros of
 // the tokens that are not there - each looks through all tokens for those of its stretch of the table - and add dP over the batch: a sort is a
 // chain of latencies that a few SMs do as fast as all of them.  (2) A warp adds a stretch of sorted places for 256 channels, rows of
 // dout read whole; a token whose places all lie in the stretch is finished there, one that began or goes on elsewhere leaves a partial row.
-// (3) Partial rows of a token are added in order.  Sums are fp32 and have one order, whatever the run: no floating-point atomics.
+// (3) Partial rows of a token are added in order.  16384 tokens, 50001 of 2048 bf16 channels: 40, 27 and 9 us (zeros of the whole table beside
+// the sort, written twice where tokens are: 40 and 49); 16384 of 256 tokens, 512 fp32 channels: 13, 8 and 4.  Sums are fp32 and have one order, whatever the run: no floating-point atomics.
 #pragma once
 #include "sa2_common.cuh"
 #include "sa2_vec8.cuh"
