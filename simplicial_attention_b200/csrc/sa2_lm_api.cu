@@ -22,10 +22,15 @@ inline int size_of(int dtype) { return dtype == SA2_BF16 ? 2 : 4; }
 inline int launch_status() { return cudaGetLastError() == cudaSuccess ? SA2_OK : SA2_ERR_CUDA; }
 inline cudaStream_t stream_of(void *s) { return reinterpret_cast<cudaStream_t>(s); }
 
+// Dynamic shared memory that kernels of varying needs are allowed: one number, since two threads may be between this and their launches
+constexpr int SMEM_LIMIT = 200 * 1024;
+template <typename K> bool allow_smem(K kernel, size_t smem) {
+    return smem <= (size_t)SMEM_LIMIT && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_LIMIT) == cudaSuccess;
+}
+
 template <typename K, typename... Args>
 int launch_clusters(K kernel, int64_t grid, int threads, size_t smem, int ctas, cudaStream_t st, const Args &...args) {
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return SA2_ERR_CUDA;
-    if (ctas > 8 && cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) return SA2_ERR_CUDA;
+    if (!allow_smem(kernel, smem)) return SA2_ERR_CUDA;
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -220,7 +225,7 @@ template <typename T> int distill_fwd(const sa2_distill_args *a, bool grad) {
     using namespace sa2::distill;
     const int warps = teacher_warps(a->k);
     const size_t smem = (size_t)warps * teacher_words(a->k) * 4;
-    if (cudaFuncSetAttribute(teacher_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return SA2_ERR_CUDA;
+    if (!allow_smem(teacher_kernel, smem)) return SA2_ERR_CUDA;
     teacher_kernel<<<(unsigned)teacher_blocks(a->rows), 32 * warps, smem, st>>>(P);
     if (int e = launch_status()) return e;
     const int g = distill_threads<T>(a->vocab);

@@ -185,3 +185,40 @@ def test_a_generation_step_as_a_graph():
         u.uniform_()
         graph.replay()
         assert torch.equal(out.clone(), step())
+
+
+def test_threads_at_once():
+    """Calls with little and with much shared memory from several threads, each on its stream: the results of calls one by one."""
+    import threading
+
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    cases = []
+    for vocab, k in ((3000, 4), (3000, 1024), (9000, 300), (40000, 32)):
+        z = torch.randn(40, vocab, generator=gen, device="cuda")
+        cases.append((z, torch.randn(40, k, generator=gen, device="cuda"), torch.randint(vocab, (40, k), generator=gen, device="cuda"),
+                      torch.rand(40, generator=gen, device="cuda")))
+
+    def run(z, t, i, u):
+        return (*sa.distillation_loss_and_grad(z, t, i), sa.sample_tokens(z, u, top_k=40, top_p=0.9))
+
+    want = [run(*c) for c in cases]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(case, expected):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(50):
+                    got = run(*case)
+                    torch.cuda.current_stream().synchronize()
+                    if not all(torch.equal(a, b) for a, b in zip(got, expected)):
+                        wrong.append("results differ")
+        except Exception as e:
+            wrong.append(repr(e))
+
+    threads = [threading.Thread(target=work, args=(c, w)) for c, w in zip(cases, want)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong, wrong[:3]
