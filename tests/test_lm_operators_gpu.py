@@ -187,6 +187,7 @@ def test_a_generation_step_as_a_graph():
         assert torch.equal(out.clone(), step())
 
 
+@pytest.mark.gpu
 def test_threads_at_once():
     """Calls with little and with much shared memory from several threads, each on its stream: the results of calls one by one."""
     import threading
