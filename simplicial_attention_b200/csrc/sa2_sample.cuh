@@ -22,6 +22,7 @@
 // 64-bit arithmetic, and the second row of an SM's two CTAs where 256 rows are no multiple of the places).
 #pragma once
 #include "sa2_common.cuh"
+#include "sa2_sample_keys.h"
 #include <cooperative_groups.h>
 #include <math_constants.h>
 
@@ -575,11 +576,7 @@ __global__ void __launch_bounds__(N, 1024 / N) kernel(const __grid_constant__ Pa
         const double least = log(fmin(min_p, 1.));
         auto stays = [&](uint32_t k) { return R.exponent(logit_of<T>(k)) >= least; };
         const float about = (float)((double)best + least * temperature);
-        if (about > -CUDART_INF_F) {
-            floor_key = min(best_key, key_of<T>(about));
-            while (floor_key > 0u && stays(floor_key - 1u)) --floor_key;
-            while (!stays(floor_key)) ++floor_key;
-        }
+        if (about > -CUDART_INF_F) floor_key = first_key(best_key, key_of<T>(about), stays);
         floor_bin = (int)fmin(-least * temperature / width + 2., (double)(N - 1));
     }
 

@@ -1,5 +1,7 @@
 """Sampled tokens against the definition in 64 bits, token for token; the inputs' random numbers come from fixed seeds, so that none lies
 within the 2^-46 of a border that the kernel's whole-number masses allow."""
+import math
+
 import pytest
 import torch
 
@@ -229,3 +231,16 @@ def test_nothing_streams_and_captured():
         graph.replay()
         want = sa.sample_tokens(z, u, top_p=0.9, top_k=1000, return_logprobs=True)
         assert torch.equal(res[0], want[0]) and torch.equal(res[1], want[1])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("vocab", [300, 5000, 140000])
+def test_floor_at_a_logit_of_zero(vocab, dtype):
+    """best + T log(min_p) cancels: the floor lies among the smallest numbers of the type.  Logits stay clear of the floor, whose last bits
+    are a matter of rounding."""
+    z, u = _logits(4, vocab, dtype)
+    z = torch.where(z.abs() < 1e-3, torch.full_like(z, 0.5), z).clamp(max=0.75)
+    for best, temperature, min_p in ((5.0, 1.0, math.exp(-5)), (1.0, 1 / math.log(2), 0.5), (7.0, 0.7, math.exp(-10))):
+        z[:, 17] = best
+        for settings in (dict(), dict(top_k=40), dict(top_p=0.9), dict(top_k=200, top_p=0.99)):
+            _check(z, u, temperature=temperature, min_p=min_p, **settings)
