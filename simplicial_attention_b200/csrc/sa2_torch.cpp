@@ -651,7 +651,7 @@ pybind11::object embed(const Tensor &tokens, const Tensor &weight, const std::op
     if ((tokens.scalar_type() != at::kLong && tokens.scalar_type() != at::kInt) || weight.dim() != 2 || dtype_of(weight) < 0 || weight.numel() == 0) return pybind11::none();
     if (tokens.numel() > INT32_MAX || weight.size(0) > INT32_MAX || weight.size(1) > INT32_MAX) return pybind11::none();
     const int64_t n = tokens.dim() ? tokens.size(-1) : 1;
-    if (positions && (positions->dim() != 2 || positions->size(1) != weight.size(1) || positions->scalar_type() != weight.scalar_type() || start < 0 || start + n > positions->size(0)))
+    if (positions && (positions->dim() != 2 || positions->size(1) != weight.size(1) || positions->scalar_type() != weight.scalar_type() || start < 0 || start > positions->size(0) - n))
         return pybind11::none();
     return pybind11::cast(Embed::apply(tokens, weight, positions, scale, start, padding));
 }

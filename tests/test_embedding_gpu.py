@@ -212,3 +212,11 @@ def test_wrong_c_calls_are_status_codes():
     lib.sa2_embed_workspace_bytes.restype = C.c_size_t
     assert lib.sa2_embed_workspace_bytes(C.c_int64(0), C.c_int32(8)) == 0
     assert lib.sa2_embed_workspace_bytes(C.c_int64(100), C.c_int32(8)) >= 4 * 400 + 4 * 2 * 8 * 4
+
+
+def test_positions_behind_the_table_are_refused():
+    tokens, weight, pos, _ = _case((2, 30), 11, 16, torch.float32, 40)
+    for start in (11, 2 ** 63 - 1, 2 ** 63 - 30):
+        with pytest.raises(ValueError, match="positions"):
+            sa.token_embedding(tokens, weight, pos, start=start)
+    assert sa.token_embedding(tokens, weight, pos, start=10).shape == (2, 30, 16)

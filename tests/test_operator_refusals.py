@@ -214,3 +214,15 @@ def test_plain_rotation_on_the_cpu():
     # scores of rows i and j depend on their distance alone
     s = lambda t: torch.einsum("bihd,bjhd->bhij", t, t)
     assert torch.allclose(s(a), s(b), atol=1e-3)
+
+
+def test_positions_behind_any_table():
+    """start + n above 2^63 is no small number."""
+    lib = _lib.lib()
+    table = dict(positions=A, dpositions=A, position_rows=100)
+    good = dict(tokens=A, weight=A, out=A, dout=A, dweight=A, workspace=A, workspace_bytes=1 << 20, rows=12, vocab=9, n=4, dim=8, padding=-1, scale=1.0)
+    for kw in (dict(start=2 ** 63 - 1), dict(start=2 ** 63 - 4), dict(start=97), dict(position_rows=-2 ** 63), dict(position_rows=3)):
+        a = EmbedArgs(**{**good, **table, **kw})
+        assert lib.sa2_embed_fwd(C.byref(a)) == 1 and lib.sa2_embed_bwd(C.byref(a)) == 1
+    with pytest.raises(ValueError, match="positions"):
+        sa.token_embedding(_cuda(2, 3, dtype=torch.long), _cuda(9, 8), _cuda(5, 8), start=2 ** 63 - 1)
