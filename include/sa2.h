@@ -352,7 +352,7 @@ size_t sa2_rotary_partial_bytes(const sa2_rotary_args *args);
  * nothing: its row of out is NaN and it has no gradient.
  * sa2_embed_bwd writes dweight (every row) and dpositions (position_rows rows, every one); either may be null.  Sums in fp32 over sorted
  * tokens, one order whatever the run.  The token `padding` (-1: none) has no gradient.  dweight and dpositions are 16-byte aligned, rows is
- * below 2^31 and a multiple of n; workspace (with dweight) of sa2_embed_workspace_bytes(), 256-byte aligned.
+ * below 2^31 and a multiple of n, vocab is below 2^31, dim up to 2^30; workspace (with dweight) of sa2_embed_workspace_bytes(), 256-byte aligned.
  */
 typedef struct sa2_embed_args {
     const void *tokens;

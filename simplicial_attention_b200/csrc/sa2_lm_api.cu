@@ -106,7 +106,7 @@ template <typename T> int rotary_dispatch(const sa2_rotary_args *a, bool backwar
 // ---------------------------------------------------------------- embedding
 int embed_check(const sa2_embed_args *a) {
     if (!a || !a->tokens || a->rows <= 0 || a->vocab <= 0 || a->n <= 0 || a->dim <= 0) return SA2_ERR_INVALID;
-    if (!known(a->dtype) || a->rows > INT32_MAX || a->vocab > INT32_MAX) return SA2_ERR_UNSUPPORTED;
+    if (!known(a->dtype) || a->rows > INT32_MAX || a->vocab > INT32_MAX || a->dim > 1 << 30) return SA2_ERR_UNSUPPORTED;
     if (a->start < 0 || a->rows % a->n) return SA2_ERR_INVALID;
     // (start + n may be above 2^63)
     if ((a->positions || a->dpositions) && (a->position_rows < a->n || a->position_rows - a->n < a->start)) return SA2_ERR_INVALID;

@@ -649,7 +649,7 @@ struct Embed : torch::autograd::Function<Embed> {
 pybind11::object embed(const Tensor &tokens, const Tensor &weight, const std::optional<Tensor> &positions, double scale, int64_t start, int64_t padding) {
     if (tracing() || !plain(weight, weight.device()) || !plain(tokens, weight.device()) || (positions && !plain(*positions, weight.device()))) return pybind11::none();
     if ((tokens.scalar_type() != at::kLong && tokens.scalar_type() != at::kInt) || weight.dim() != 2 || dtype_of(weight) < 0 || weight.numel() == 0) return pybind11::none();
-    if (tokens.numel() > INT32_MAX || weight.size(0) > INT32_MAX || weight.size(1) > INT32_MAX) return pybind11::none();
+    if (tokens.numel() > INT32_MAX || weight.size(0) > INT32_MAX || weight.size(1) > 1 << 30) return pybind11::none();
     const int64_t n = tokens.dim() ? tokens.size(-1) : 1;
     if (positions && (positions->dim() != 2 || positions->size(1) != weight.size(1) || positions->scalar_type() != weight.scalar_type() || start < 0 || start > positions->size(0) - n))
         return pybind11::none();

@@ -38,6 +38,8 @@ def token_embedding(tokens: Tensor, weight: Tensor, pos_weight: Tensor | None = 
         raise ValueError("the tables must share one dtype, float32 or bfloat16")
     if any(t.dim() != 2 for t in tensors[1:]) or weight.numel() == 0 or any(t.shape[1] != weight.shape[1] for t in tensors[1:]):
         raise ValueError("expected tables of (rows, dim), with one dim and at least one row")
+    if weight.shape[1] > 2 ** 30:
+        raise ValueError("rows of a table may have up to 2^30 channels")
     if pos_weight is not None and not 0 <= start <= pos_weight.shape[0] - (tokens.shape[-1] if tokens.dim() else 1):
         raise ValueError("the positions do not fit the table of positions")
     raise RuntimeError("token_embedding takes plain tensors of one device, outside of tracing and transforms")

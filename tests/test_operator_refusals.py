@@ -226,3 +226,14 @@ def test_positions_behind_any_table():
         assert lib.sa2_embed_fwd(C.byref(a)) == 1 and lib.sa2_embed_bwd(C.byref(a)) == 1
     with pytest.raises(ValueError, match="positions"):
         sa.token_embedding(_cuda(2, 3, dtype=torch.long), _cuda(9, 8), _cuda(5, 8), start=2 ** 63 - 1)
+
+
+def test_widths_next_to_the_largest_int():
+    """Pieces of a row are counted in 32 bits."""
+    lib = _lib.lib()
+    good = dict(tokens=A, weight=A, out=A, dout=A, dweight=A, workspace=A, workspace_bytes=1 << 62, rows=12, vocab=9, n=4, dim=8, padding=-1, scale=1.0)
+    for dim in (2 ** 30 + 1, 2 ** 31 - 128, 2 ** 31 - 1):
+        a = EmbedArgs(**{**good, "dim": dim})
+        assert lib.sa2_embed_fwd(C.byref(a)) == 2 and lib.sa2_embed_bwd(C.byref(a)) == 2
+    with pytest.raises(ValueError, match="2\\^30"):
+        sa.token_embedding(_cuda(2, 3, dtype=torch.long), _cuda(1, 2 ** 30 + 8))
