@@ -382,7 +382,8 @@ size_t sa2_embed_workspace_bytes(int64_t rows, int32_t dim);
  * zero.  Rows are strided, their elements contiguous; logits and dlogits fp32 or bf16 (dtype), teacher fp32 or bf16, index int64 or int32.
  * sa2_distill_fwd writes row_loss, and total: the sum of row_loss over `reduction` (SA2_SUM: 1, SA2_MEAN: the number of rows with
  * entries, at least 1); either may be null.  The workspace (sa2_distill_workspace_bytes(), 256-byte aligned) keeps what sa2_distill_bwd needs
- * beside the logits; gout is the gradient of the total, or of every row (gout_rows != 0), null is 1.  sa2_distill_both is the forward and
+ * beside the logits, whatever the forward was asked for; gout is the gradient of the total of this call's `reduction`, or of every row
+ * (gout_rows != 0), null is 1.  sa2_distill_both is the forward and
  * the backward for gout = grad_scale, which reads the logits from memory once.
  * dlogits must not overlap logits.
  */

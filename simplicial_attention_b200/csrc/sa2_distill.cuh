@@ -37,8 +37,8 @@ struct Params {
     float *row_loss;            // [rows]
     void *dz;                   // [rows][vocab], row stride ds
     const float *gout;          // gradient of the loss: one, or one for each row (gs = 1); null: 1
-    float *scale;               // two factors more: 1 / rows that count (or null), and one of the caller
-    float times;
+    float *scale;               // 1 / rows that count, from total_kernel; -1 while that has not run.  bwd_kernel: null if the loss is no mean
+    float times;                // a factor of the caller
     int64_t rows, zs, ts, is, ds;
     int vocab, k, gs;
     int index64, teacher_bf16;
@@ -279,6 +279,7 @@ __global__ void __launch_bounds__(1024) teacher_kernel(const __grid_constant__ P
     if (threadIdx.x == 0) {
         for (int w = 1; w < (int)blockDim.x / 32; ++w) rows += of_warp[w];
         P.counts[blockIdx.x] = rows;
+        if (blockIdx.x == 0) *P.scale = -1.f;
     }
 }
 // An entry's part of a row's loss over T^2, without `self`
@@ -478,7 +479,7 @@ __global__ void __launch_bounds__(G, 1024 / G) both_kernel(const __grid_constant
     }
 }
 
-// out: sum of the rows' losses, over the rows that count if `mean`; factor: of the gradient that goes with it
+// out: sum of the rows' losses, over the rows that count if `mean`; factor: 1 / these rows, for the gradient of a mean
 __global__ void __launch_bounds__(1024) total_kernel(const float *row_loss, const int *counts, int64_t rows, int mean, float *out, float *factor) {
     __shared__ double sums[32];
     __shared__ long long count_of[32];
@@ -502,8 +503,17 @@ __global__ void __launch_bounds__(1024) total_kernel(const float *row_loss, cons
             c += count_of[w];
         }
         *out = (float)(mean ? s / (double)(c > 0 ? c : 1) : s);
-        *factor = mean ? 1.f / (float)(c > 0 ? c : 1) : 1.f;
+        *factor = 1.f / (float)(c > 0 ? c : 1);
     }
+}
+
+// 1 / rows that count, in each lane of a warp: for a backward whose forward was not asked for their total
+__device__ __noinline__ float count_again(const int *counts, int64_t rows) {
+    long long c = 0;
+    for (int64_t x = threadIdx.x & 31; x < (rows + TEACHER_ROWS - 1) / TEACHER_ROWS; x += 32) c += counts[x];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) c += __shfl_xor_sync(0xffffffffu, c, o);
+    return 1.f / (float)(c > 0 ? c : 1);
 }
 
 template <typename T, int G>
@@ -513,7 +523,9 @@ __global__ void __launch_bounds__(G == 32 ? 256 : G, G == 32 ? 4 : 1536 / G) bwd
     const T *row = reinterpret_cast<const T *>(P.z) + r * P.zs;
     T *grad = reinterpret_cast<T *>(P.dz) + r * P.ds;
     const bool there = P.there[r];
-    const float coef = there ? (P.gout ? P.gout[r * P.gs] : 1.f) * (P.scale ? P.scale[0] : 1.f) * P.times * P.t : 0.f;
+    float part = P.scale ? *P.scale : 1.f;
+    if (part < 0.f) part = count_again(P.counts, P.rows);
+    const float coef = there ? (P.gout ? P.gout[r * P.gs] : 1.f) * part * P.times * P.t : 0.f;
     const float best = there ? P.stats[2 * r] : 0.f, inv = there ? 1.f / P.stats[2 * r + 1] : 0.f;
     const Factor f = factor(P);
     gradient<G, T, 4, false>(row, grad, P.vocab, there, best, coef * inv, f);

@@ -301,3 +301,34 @@ def test_the_loss_is_the_callers_and_no_second_backward():
     assert torch.equal(torch.autograd.grad(loss, leaf, retain_graph=True)[0], want)
     with pytest.raises(RuntimeError, match="create_graph"):
         torch.autograd.grad(loss, leaf, create_graph=True)
+
+
+@pytest.mark.parametrize("vocab", [300, 5001])
+@pytest.mark.parametrize("asked", ["row_loss", "total", "both"])
+@pytest.mark.parametrize("forward, backward", [(0, 0), (0, 1), (1, 0), (1, 1)], ids=str)
+def test_c_calls_in_any_order(vocab, asked, forward, backward):
+    """The gradient of a sum (0) or a mean (1), whatever loss the forward was asked for, from a workspace that held something else."""
+    import ctypes as C
+
+    from simplicial_attention_b200 import _lib
+    from test_operator_refusals import DistillArgs
+    z, t, i = _inputs(70, vocab, 5, torch.float32)
+    i[::3] = -1
+    lib = _lib.lib()
+    lib.sa2_distill_workspace_bytes.restype = C.c_size_t
+    ws = torch.full((lib.sa2_distill_workspace_bytes(C.c_int64(70), C.c_int32(5)),), 0x41, dtype=torch.uint8, device="cuda")
+    row_loss, total, grad = torch.empty(70, device="cuda"), torch.empty((), device="cuda"), torch.empty_like(z)
+    a = DistillArgs(logits=z.data_ptr(), teacher=t.data_ptr(), index=i.data_ptr(), dlogits=grad.data_ptr(), workspace=ws.data_ptr(), workspace_bytes=ws.numel(), rows=70,
+                    logits_stride=vocab, teacher_stride=5, index_stride=5, dlogits_stride=vocab, vocab=vocab, k=5, index64=1, reduction=forward, temperature=1.5,
+                    grad_scale=1.0, stream=torch.cuda.current_stream().cuda_stream)
+    a.row_loss = row_loss.data_ptr() if asked != "total" else None
+    a.total = total.data_ptr() if asked != "row_loss" else None
+    assert lib.sa2_distill_fwd(C.byref(a)) == 0
+    a.reduction = backward
+    assert lib.sa2_distill_bwd(C.byref(a)) == 0
+    leaf = z.requires_grad_()
+    loss = lambda reduction: sa.distillation_loss(z.detach(), t, i, temperature=1.5, reduction=reduction)
+    assert asked == "total" or torch.equal(row_loss, loss("none"))
+    assert asked == "row_loss" or torch.equal(total, loss(("sum", "mean")[forward]))
+    want = torch.autograd.grad(sa.distillation_loss(leaf, t, i, temperature=1.5, reduction=("sum", "mean")[backward]), leaf)[0]
+    assert torch.equal(grad, want) and (grad[1::3] != 0).any()
