@@ -192,7 +192,7 @@ class TwoSimplicialLM(Module):
             k = max(1, math.ceil((1 - filter_thres) * logits.shape[-1]))
             val, ind = torch.topk(logits, k)
             kept = torch.full_like(logits, float("-inf")).scatter_(-1, ind, val)
-            noise = -torch.log(-torch.log(torch.rand_like(kept).clamp_min(1e-20)).clamp_min(1e-20))
+            noise = -torch.log((-torch.log(torch.rand_like(kept).clamp_min(1e-20))).clamp_min(1e-20))
             nxt = (kept / max(temperature, 1e-10) + noise).argmax(dim=-1, keepdim=True)
             out = torch.cat((out, nxt), dim=-1)
         return out[..., prompt.shape[-1]:]

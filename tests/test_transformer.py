@@ -121,3 +121,32 @@ def test_stack_matches_the_reference_stack_with_shared_weights():
             got = net(x).cpu()
         err = (got - want).abs().max().item() / want.abs().max().item()
         assert err <= 1e-4, (fused, err)
+
+
+class _KnownLogits(TwoSimplicialLM):
+    """A model whose next token's logits do not depend on its input."""
+
+    def __init__(self, logits):
+        super().__init__(num_tokens=logits.numel(), dim=8, depth=1, dim_head=8, heads=1, transformer_kwargs=dict(key_value_heads=1))
+        self.known = logits
+
+    def forward(self, x, cache=None, return_cache=False):
+        logits = self.known.expand(*x.shape, -1)
+        return (logits, {}) if return_cache else logits
+
+
+@pytest.mark.parametrize("use_cache", [True, False])
+@pytest.mark.parametrize("temperature", [1.0, 0.5])
+def test_sampled_frequencies(temperature, use_cache):
+    """Gumbel noise on the three largest of six logits draws from their softmax."""
+    torch.manual_seed(9)
+    z = torch.tensor([2.0, 0.0, 1.0, -1.0, float("-inf"), 1.5])
+    n = 20000
+    out = _KnownLogits(z).sample(torch.zeros(n, 2, dtype=torch.long), 5, temperature=temperature, filter_thres=0.5, use_cache=use_cache)
+    w = torch.exp(z / temperature)
+    w[[1, 3, 4]] = 0
+    for column in out.unbind(1):
+        got = torch.bincount(column, minlength=6) / n
+        assert (got[w == 0] == 0).all()
+        assert (got - w / w.sum()).abs().max() <= 5 * 0.5 / n ** 0.5     # five standard deviations
+    assert not torch.equal(out[:, 0], out[:, 1])
