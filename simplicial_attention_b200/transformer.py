@@ -171,7 +171,8 @@ class TwoSimplicialLM(Module):
         until ``seq_len`` tokens, returning only the generated part.  With ``use_cache`` the prompt is run
         once and every further token costs one position: the standard layers keep their keys and values,
         the simplicial layers only their ``w1 - 1`` / ``w2 - 1`` row windows.  With any of ``top_k``, ``top_p`` and ``min_p`` the tokens
-        come from ``sample_tokens`` (``filter_thres`` is then not used), its uniform numbers from ``generator``."""
+        come from ``sample_tokens`` (``filter_thres`` is then not used; it needs CUDA and fp32 or bf16 logits).  Random numbers come from
+        ``generator``, or torch's own."""
         filtered = top_k is not None or top_p is not None or min_p is not None
         out = prompt.clone()
         steps = max(0, seq_len - prompt.shape[-1])
@@ -192,7 +193,8 @@ class TwoSimplicialLM(Module):
             k = max(1, math.ceil((1 - filter_thres) * logits.shape[-1]))
             val, ind = torch.topk(logits, k)
             kept = torch.full_like(logits, float("-inf")).scatter_(-1, ind, val)
-            noise = -torch.log((-torch.log(torch.rand_like(kept).clamp_min(1e-20))).clamp_min(1e-20))
+            uniform = torch.rand(kept.shape, device=kept.device, generator=generator)
+            noise = -torch.log((-torch.log(uniform.clamp_min(1e-20))).clamp_min(1e-20))
             nxt = (kept / max(temperature, 1e-10) + noise).argmax(dim=-1, keepdim=True)
             out = torch.cat((out, nxt), dim=-1)
         return out[..., prompt.shape[-1]:]

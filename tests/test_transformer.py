@@ -150,3 +150,15 @@ def test_sampled_frequencies(temperature, use_cache):
         assert (got[w == 0] == 0).all()
         assert (got - w / w.sum()).abs().max() <= 5 * 0.5 / n ** 0.5     # five standard deviations
     assert not torch.equal(out[:, 0], out[:, 1])
+
+
+@pytest.mark.parametrize("filters", [dict(), pytest.param(dict(top_p=0.9), marks=pytest.mark.gpu)], ids=["default", "top_p"])
+def test_sampling_draws_from_the_generator(filters):
+    device = "cuda" if filters else "cpu"
+    model = _KnownLogits(torch.zeros(50, device=device))
+    prompt = torch.zeros(4, 2, dtype=torch.long, device=device)
+    draw = lambda seed: model.sample(prompt, 12, filter_thres=0.0, generator=torch.Generator(device=device).manual_seed(seed), **filters)
+    state = torch.cuda.get_rng_state() if filters else torch.get_rng_state()
+    a = draw(1)
+    assert torch.equal(a, draw(1)) and not torch.equal(a, draw(2))
+    assert torch.equal(state, torch.cuda.get_rng_state() if filters else torch.get_rng_state())      # and from nothing else
