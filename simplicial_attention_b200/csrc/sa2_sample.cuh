@@ -645,7 +645,10 @@ __global__ void __launch_bounds__(N, 1024 / N) kernel(const __grid_constant__ Pa
     // Top-p of the whole row: a sum in fp32 says what the row's mass is to a ten thousandth, which mostly shows the cut already.  With min-p
     // the first round does without the histogram: what min-p leaves is mostly little, and holds the cut or needs none.
     const bool of_row = by_mass && !by_count, cuts = by_count || by_mass;
-    bool count = cuts && !small && !(of_row && first_list), near = small;            // near: at most N logits are left
+    // Both take differences of logits in fp32.  Where one beyond fp32 may lie in a stretch, or have a mass (T above 1e37), there is neither: exact
+    // masses, and a cut among all keys.
+    const bool wide = fmax(width * N, nats * temperature) > 3.4e38;
+    bool count = cuts && !small && !(of_row && first_list) && !wide, near = small;   // near: at most N logits are left
     unsigned long long least = 0ull, most = 0ull;        // bounds of the row's mass
     for (bool again = false;; again = true) {
         if (count || of_row || first_list) {
@@ -679,7 +682,7 @@ __global__ void __launch_bounds__(N, 1024 / N) kernel(const __grid_constant__ Pa
                 near = near || n <= (unsigned long long)N;
             }
         }
-        if (again || near || count || !cuts) break;
+        if (again || near || count || !cuts || wide) break;
         count = true;
     }
     if (count) {
@@ -694,7 +697,7 @@ __global__ void __launch_bounds__(N, 1024 / N) kernel(const __grid_constant__ Pa
         S.total[threadIdx.x] = c;
     }
     // (a temperature whose inverse is no fp32 number left that sum without meaning)
-    if (of_row && R.inv_t > 1e38) least = most = row_mass();
+    if (of_row && (R.inv_t > 1e38 || wide)) least = most = row_mass();
     // The keys between which a cut lies, from the stretches [first, last]: of the numbers that are not outside of them, so that no more than one
     // stretch more is between the two keys.  Margins: a logit's stretch is found in fp32.
     auto key_from = [&](int last) {
@@ -734,7 +737,7 @@ __global__ void __launch_bounds__(N, 1024 / N) kernel(const __grid_constant__ Pa
             if (by_count) cut = find_cut(R, V, S, rank, ctas, from, max(from, to), by_mass, (unsigned long long)top_k, 0ull);
             if (by_mass) {
                 const unsigned long long want = wanted_mass(top_p, cut.mass);
-                if (by_count) {
+                if (by_count && count) {
                     bracket(S, width, R.inv_t, true, (double)want / one, (double)want / one);
                     from = max(from, key_from(S.last_bin));
                     to = key_to(S.first_bin);

@@ -2,6 +2,7 @@
 within the 2^-46 of a border that the kernel's whole-number masses allow."""
 import math
 
+import numpy as np
 import pytest
 import torch
 
@@ -244,3 +245,43 @@ def test_floor_at_a_logit_of_zero(vocab, dtype):
         z[:, 17] = best
         for settings in (dict(), dict(top_k=40), dict(top_p=0.9), dict(top_k=200, top_p=0.99)):
             _check(z, u, temperature=temperature, min_p=min_p, **settings)
+
+
+def _tokens_of_long_sums(logits, uniform, temperature, top_k=None, top_p=None, min_p=None):
+    """As _oracle, with sums of 64-bit significands.  A thousand equal logits and two thousand of a weight of 4e-14 have 1000 + 8.7e-11, which
+    a sum in fp64 takes for 1000; the 701st token stays for a top_p of 0.7 all the same: 700 is less than 0.7 (1000 + 8.7e-11)."""
+    tokens = []
+    for r, z in enumerate(logits.double().cpu().numpy()):
+        if np.isnan(z).any() or np.isinf(z.max()):
+            tokens.append(-1)
+            continue
+        w = np.exp(((z - z.max()) / temperature).astype(np.longdouble))
+        order = np.lexsort((np.arange(z.size), -z))
+        count = z.size if top_k is None else min(top_k, z.size)
+        if top_p is not None:
+            mass = w[order[:count]].cumsum()
+            count = min(count, 1 + int((mass < np.longdouble(top_p) * mass[-1]).sum()))
+        keep = np.zeros(z.size, dtype=bool)
+        keep[order[:count]] = True
+        if min_p is not None:
+            keep &= w >= min_p
+        mass = (w * keep).cumsum()
+        tokens.append(min(int((mass <= np.longdouble(uniform[r].item()) * mass[-1]).sum()), int(keep.nonzero()[0].max())))
+    return tokens
+
+
+@pytest.mark.parametrize("vocab", [200, 3000, 70000])
+def test_rows_that_span_more_than_fp32(vocab):
+    """best - v is no fp32 number, and at these temperatures v has a mass all the same."""
+    _, u = _logits(4, vocab, torch.float32)
+    z = torch.full((4, vocab), -3e38, device="cuda")
+    z[0, ::2] = 3e38
+    z[1] = torch.linspace(-3.3e38, 3.3e38, vocab, device="cuda")
+    z[2, 1::2] = torch.finfo(torch.float32).max
+    z[2, ::2] = torch.finfo(torch.float32).min
+    z[3, : vocab // 3] = 1e38
+    for t in (3e36, 9e36, 1e37, 1.3e37, 1e38, 3e38):
+        for settings in (dict(), dict(top_k=vocab * 5 // 7), dict(top_k=vocab // 3), dict(top_p=0.9999), dict(top_p=0.7), dict(top_k=vocab * 5 // 7, top_p=0.95), dict(min_p=0.01),
+                         dict(min_p=0.001, top_p=0.99)):
+            for x in (z, z[:1].bfloat16()):
+                assert sa.sample_tokens(x, u[:x.shape[0]], temperature=t, **settings).tolist() == _tokens_of_long_sums(x, u, t, **settings)
