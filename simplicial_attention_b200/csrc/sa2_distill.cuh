@@ -9,8 +9,9 @@
 // reading z and writing dz (backward) once.  The forward keeps the running maximum of what a thread has seen and the sum of exponentials
 // against it; per bf16 logit a fused product, ex2 and an addition, which 16 ex2 per clock and SM allow at the rate the loads come.  4095
 // rows of 32000 fp32 logits: forward 100 us (5.2 TB/s), backward 163 (6.4 TB/s, a copy's rate); 16384 rows of 256: 18 the teacher, 12, 9.
-// Sums over a row are fp32 and have one order; the row's K terms, and the sum over rows, are 64 bits: they are few, and
-// log p - log q cancels where the student is good.
+// A row's sum s of exponentials is fp32 and has one order.  The rest of its loss is formed in 64 bits, as  sum_k p_k log p_k + log s -
+// sum_k p_k (z_k - max) / T:  it is little, and cancels where the student is good.  What is left then is the rounding of s, at most some 2^-21, and that of
+// the p_k of the last sum (fp32, 2^-24 each), times T^2.
 #pragma once
 #include "sa2_common.cuh"
 #include "sa2_vec8.cuh"
@@ -30,7 +31,7 @@ struct Params {
     // what teacher_kernel makes of them
     int *place;                 // [rows][k]: -1 where an entry is not there, has no mass, or names the token of an earlier one
     float *prob;                // [rows][k]: of the token
-    float *self;                // [rows]: sum of p log p
+    double *self;               // [rows]: sum of p log p
     int *there;                 // [rows]: whether the row counts
     int *counts;                // rows that count, of every TEACHER_ROWS
     float *stats;               // [rows][2]: maximum of z, sum of exp((z - maximum) / T)
@@ -268,7 +269,7 @@ __global__ void __launch_bounds__(1024) teacher_kernel(const __grid_constant__ P
         }
         __syncwarp();
         if (lane == 0) {
-            P.self[r] = (float)self;
+            P.self[r] = self;
             P.there[r] = counted;
         }
         rows += counted;
@@ -282,10 +283,9 @@ __global__ void __launch_bounds__(1024) teacher_kernel(const __grid_constant__ P
         if (blockIdx.x == 0) *P.scale = -1.f;
     }
 }
-// An entry's part of a row's loss over T^2, without `self`
-__device__ __forceinline__ double term(float prob, float logit, float best, double log_s, double inv_t) {
-    return (double)prob * (log_s - ((double)logit - (double)best) * inv_t);
-}
+// An entry's part of the last sum of a row's loss
+__device__ __forceinline__ double term(float prob, float logit, float best, double inv_t) { return (double)prob * (((double)logit - (double)best) * inv_t); }
+__device__ __forceinline__ float row_loss(double self, float s, double terms, float t) { return (float)((self + log((double)s) - terms) * (double)t * (double)t); }
 
 // Running maximum and sum of exponentials of what a thread has seen
 template <typename T> struct Running {
@@ -392,17 +392,17 @@ __global__ void __launch_bounds__(G == 32 ? 256 : G, G == 32 ? 4 : 1536 / G) fwd
     }
     const float2 all = joined<G, T>(run.result(), of_warp, f);
     const float best = all.x == -CUDART_INF_F ? 0.f : all.x, s = all.y;
-    const double log_s = log((double)s), inv_t = 1. / (double)P.t;
-    double loss = 0.;
+    const double inv_t = 1. / (double)P.t;
+    double terms = 0.;
     for (int k = Group<G>::rank(); k < P.k; k += G) {
         const int i = P.place[r * P.k + k];
-        if (i >= 0) loss += term(P.prob[r * P.k + k], (float)row[i], best, log_s, inv_t);
+        if (i >= 0) terms += term(P.prob[r * P.k + k], (float)row[i], best, inv_t);
     }
-    loss = Group<G>::reduce(loss, scratch, [](double a, double b) { return a + b; });
+    terms = Group<G>::reduce(terms, scratch, [](double a, double b) { return a + b; });
     if (Group<G>::rank() == 0) {
         P.stats[2 * r] = best;
         P.stats[2 * r + 1] = s;
-        P.row_loss[r] = (float)((loss + (double)P.self[r]) * (double)P.t * (double)P.t);
+        P.row_loss[r] = row_loss(P.self[r], s, terms, P.t);
     }
 }
 
@@ -416,7 +416,7 @@ template <typename T, int G>
 __global__ void __launch_bounds__(G, 1024 / G) both_kernel(const __grid_constant__ Params P) {
     __shared__ float2 of_warp[G / 32];
     __shared__ int counted[G / 32];
-    __shared__ double loss_of[G / 32];
+    __shared__ double terms_of[G / 32];
     const int warp = threadIdx.x >> 5;
     const int64_t r = blockIdx.x;
     const T *row = reinterpret_cast<const T *>(P.z) + r * P.zs;
@@ -456,8 +456,8 @@ __global__ void __launch_bounds__(G, 1024 / G) both_kernel(const __grid_constant
     // the teacher's tokens and the loss
     const bool on = there && warp * 32 < P.k;
     if (on) {
-        const double log_s = log((double)s), inv_t = 1. / (double)P.t;
-        double loss = 0.;
+        const double inv_t = 1. / (double)P.t;
+        double terms = 0.;
         for (int k = threadIdx.x; k < P.k; k += G) {
             if (k >= G) {
                 place = P.place[r * P.k + k];
@@ -466,16 +466,16 @@ __global__ void __launch_bounds__(G, 1024 / G) both_kernel(const __grid_constant
             }
             if (place < 0) continue;
             grad[place] = (T)(coef * (weight<T>(logit - best, f) * inv - prob));
-            loss += term(prob, logit, best, log_s, inv_t);
+            terms += term(prob, logit, best, inv_t);
         }
-        loss = Group<32>::reduce(loss, (double *)nullptr, [](double a, double b) { return a + b; });
-        if (threadIdx.x % 32 == 0) loss_of[warp] = loss;
+        terms = Group<32>::reduce(terms, (double *)nullptr, [](double a, double b) { return a + b; });
+        if (threadIdx.x % 32 == 0) terms_of[warp] = terms;
     }
     __syncthreads();
     if (threadIdx.x == 0) {
-        double loss = there ? (double)P.self[r] : 0.;
-        for (int w = 0; there && w < G / 32 && w * 32 < P.k; ++w) loss += loss_of[w];
-        P.row_loss[r] = (float)(loss * (double)P.t * (double)P.t);
+        double terms = 0.;
+        for (int w = 0; there && w < G / 32 && w * 32 < P.k; ++w) terms += terms_of[w];
+        P.row_loss[r] = there ? row_loss(P.self[r], s, terms, P.t) : 0.f;
     }
 }
 
@@ -540,7 +540,7 @@ __global__ void __launch_bounds__(G == 32 ? 256 : G, G == 32 ? 4 : 1536 / G) bwd
 inline size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
 inline int64_t teacher_blocks(int64_t rows) { return (rows + TEACHER_ROWS - 1) / TEACHER_ROWS; }
 inline size_t workspace_bytes(int64_t rows, int k) {
-    return 2 * up256((size_t)rows * k * 4) + 3 * up256((size_t)rows * 4) + up256((size_t)rows * 8) + up256((size_t)teacher_blocks(rows) * 4) + 256;
+    return 2 * up256((size_t)rows * k * 4) + 2 * up256((size_t)rows * 4) + 2 * up256((size_t)rows * 8) + up256((size_t)teacher_blocks(rows) * 4) + 256;
 }
 inline void carve(Params &P, void *workspace) {
     char *p = reinterpret_cast<char *>(workspace);
@@ -551,7 +551,7 @@ inline void carve(Params &P, void *workspace) {
     };
     P.place = reinterpret_cast<int *>(take((size_t)P.rows * P.k * 4));
     P.prob = reinterpret_cast<float *>(take((size_t)P.rows * P.k * 4));
-    P.self = reinterpret_cast<float *>(take((size_t)P.rows * 4));
+    P.self = reinterpret_cast<double *>(take((size_t)P.rows * 8));
     P.there = reinterpret_cast<int *>(take((size_t)P.rows * 4));
     P.stats = reinterpret_cast<float *>(take((size_t)P.rows * 8));
     P.counts = reinterpret_cast<int *>(take((size_t)teacher_blocks(P.rows) * 4));

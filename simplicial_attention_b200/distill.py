@@ -41,7 +41,9 @@ def distillation_loss(logits: Tensor, teacher_logits: Tensor, teacher_index: Ten
     ``logits``: ``(..., vocab)``, fp32 or bf16; ``teacher_logits``, ``teacher_index``: ``(..., k)``, k up to 1024.  Entries whose index lies
     outside ``[0, vocab)`` (say -1) are not there, whatever their logit; a row without entries, or whose entries are all -inf, has loss
     and gradient zero and does not count in the mean.  Entries of one token add up.  The result is fp32: the mean over the rows that
-    count (0 if none does), their ``"sum"``, or with ``"none"`` one value for each row.  Gradients flow to ``logits``."""
+    count (0 if none does), their ``"sum"``, or with ``"none"`` one value for each row.  Gradients flow to ``logits``.
+
+    A row's sum of exponentials is fp32: however near the student is to its teacher, the loss is good to about ``2^-21 T^2``, no better."""
     _check(temperature, reduction, _REDUCTIONS)
     loss = _lib.ext().distill(logits, teacher_logits, teacher_index, float(temperature), _REDUCTIONS[reduction])
     return loss if loss is not None else _refuse(logits, teacher_logits, teacher_index, temperature, reduction, _REDUCTIONS)

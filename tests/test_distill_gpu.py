@@ -332,3 +332,22 @@ def test_c_calls_in_any_order(vocab, asked, forward, backward):
     assert asked == "row_loss" or torch.equal(total, loss(("sum", "mean")[forward]))
     want = torch.autograd.grad(sa.distillation_loss(leaf, t, i, temperature=1.5, reduction=("sum", "mean")[backward]), leaf)[0]
     assert torch.equal(grad, want) and (grad[1::3] != 0).any()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("temperature", [1.0, 20.0, 100.0])
+@pytest.mark.parametrize("vocab, k", [(256, 256), (1024, 1024), (3000, 500), (20000, 1000), (70000, 256)], ids=str)
+def test_a_student_next_to_its_teacher(vocab, k, temperature, dtype):
+    """k equal logits and nothing else, so that the row's sum is k without a rounding; a teacher that is flat but for a tenth.  What the loss is
+    made of cancels to its 10^-4 and less: it is formed in 64 bits (10^-13 for a few hundred roundings of numbers below ten) and rounded once."""
+    gen = torch.Generator(device="cuda").manual_seed(k)
+    z = torch.full((20, vocab), float("-inf"), device="cuda", dtype=dtype)
+    z[:, :k] = 0.0
+    t = 0.1 * torch.randn(20, k, generator=gen, device="cuda")
+    i = torch.stack([torch.randperm(k, generator=gen, device="cuda") for _ in range(20)])
+    want = _oracle(z, t, i, temperature)[0]
+    bound = want.abs() * 2 * U + temperature ** 2 * 1e-13
+    got = sa.distillation_loss(z, t, i, temperature=temperature, reduction="none")
+    assert ((got.double() - want).abs() <= bound).all()
+    for total in (sa.distillation_loss(z, t, i, temperature=temperature), sa.distillation_loss_and_grad(z, t, i, temperature=temperature)[0]):
+        assert (total.double() - want.mean()).abs() <= bound.mean() + want.mean().abs() * 2 * U
