@@ -283,8 +283,11 @@ __global__ void __launch_bounds__(1024) teacher_kernel(const __grid_constant__ P
         if (blockIdx.x == 0) *P.scale = -1.f;
     }
 }
-// An entry's part of the last sum of a row's loss
-__device__ __forceinline__ double term(float prob, float logit, float best, double inv_t) { return (double)prob * (((double)logit - (double)best) * inv_t); }
+// An entry's part of the last sum of a row's loss; -inf for a token that the student rules out, also where the probability is 0 in fp32
+__device__ __forceinline__ double term(float prob, float logit, float best, double inv_t) {
+    const double x = ((double)logit - (double)best) * inv_t;
+    return x == -CUDART_INF ? x : (double)prob * x;
+}
 __device__ __forceinline__ float row_loss(double self, float s, double terms, float t) { return (float)((self + log((double)s) - terms) * (double)t * (double)t); }
 
 // Running maximum and sum of exponentials of what a thread has seen

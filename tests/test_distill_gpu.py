@@ -351,3 +351,21 @@ def test_a_student_next_to_its_teacher(vocab, k, temperature, dtype):
     assert ((got.double() - want).abs() <= bound).all()
     for total in (sa.distillation_loss(z, t, i, temperature=temperature), sa.distillation_loss_and_grad(z, t, i, temperature=temperature)[0]):
         assert (total.double() - want.mean()).abs() <= bound.mean() + want.mean().abs() * 2 * U
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("vocab", [300, 5001])
+@pytest.mark.parametrize("below", [50.0, 104.0, 300.0, 740.0])
+def test_ruled_out_tokens_of_little_probability(below, vocab, dtype):
+    """An entry `below` nats under the best has a probability of exp(-below), 0 in fp32 from 104 on; the student's -inf there makes the loss inf."""
+    z, t, i = _inputs(4, vocab, 5, dtype)
+    t[:, 0], t[:, 1:] = 0.0, -below
+    z[1, i[1, 3]] = float("-inf")
+    loss = sa.distillation_loss(z, t, i, reduction="none")
+    assert torch.equal(loss == float("inf"), torch.tensor([False, True, False, False], device="cuda")) and not loss.isnan().any()
+    leaf = z.requires_grad_()
+    grad = torch.autograd.grad(sa.distillation_loss(leaf, t, i), leaf)[0]
+    total, both = sa.distillation_loss_and_grad(z.detach(), t, i)
+    assert total == float("inf") and grad.isfinite().all() and both.isfinite().all()
+    keep = [0, 2, 3]
+    _check(z.detach()[keep], t[keep], i[keep], 1.0, "none")
