@@ -66,19 +66,28 @@ def qk_norm_rotary(q: Tensor, k: Tensor, q_weight: Tensor, k_weight: Tensor, fre
     raise RuntimeError("qk_norm_rotary takes plain tensors of one device (up to 2^30 rows, 4096 heads), outside of tracing and transforms")
 
 
-def _plain(q, k, q_weight, k_weight, freqs, start, eps, interleaved=False):
-    """The same in torch's operators: CPU tensors, other head dims, and what torch records or transforms."""
-    steps = torch.arange(start, start + q.shape[1], device=q.device)[:, None, None] * freqs      # modulo a turn: int64 wraps
+def _turned(n, freqs, start, interleaved=False):
+    """The rotation of rows at positions ``start`` on, in torch's operators: a function of fp32 heads ``(b, n, heads, d)``."""
+    steps = torch.arange(start, start + n, device=freqs.device)[:, None, None] * freqs      # modulo a turn: int64 wraps
     angle = steps.double() * (math.pi * 2.0 ** -63)
     cos, sin = angle.cos().float(), angle.sin().float()
     rotated = 2 * freqs.numel()
 
-    def one(x, weight):
-        y = x.float()
-        y = y * torch.rsqrt(y.square().mean(-1, keepdim=True) + eps) * weight.float()
+    def turn(y):
         a, b = (y[..., 0:rotated:2], y[..., 1:rotated:2]) if interleaved else y[..., :rotated].chunk(2, -1)
         a, b = a * cos - b * sin, b * cos + a * sin
         turned = torch.stack((a, b), dim=-1).flatten(-2) if interleaved else torch.cat((a, b), dim=-1)
-        return torch.cat((turned, y[..., rotated:]), dim=-1).to(x.dtype)
+        return torch.cat((turned, y[..., rotated:]), dim=-1)
+
+    return turn
+
+
+def _plain(q, k, q_weight, k_weight, freqs, start, eps, interleaved=False):
+    """The same in torch's operators: CPU tensors, other head dims, and what torch records or transforms."""
+    turn = _turned(q.shape[1], freqs, start, interleaved)
+
+    def one(x, weight):
+        y = x.float()
+        return turn(y * torch.rsqrt(y.square().mean(-1, keepdim=True) + eps) * weight.float()).to(x.dtype)
 
     return one(q, q_weight), one(k, k_weight)

@@ -29,8 +29,14 @@ from .distill import distillation_loss, distillation_loss_and_grad
 from .headnorm import RMSNorm
 from .mha import SlidingWindowTwoSimplicialMHA, _child
 from .rotary import _plain as plain_qk_norm_rotary
+from .rotary import _turned as turned
 from .rotary import rotary_frequencies
 from .sampling import sample_tokens
+
+
+def _hooked(m):
+    """Whether a call of ``m`` runs more than its class's ``forward``."""
+    return bool(m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks or "forward" in m.__dict__)
 
 
 class Attention(Module):
@@ -51,8 +57,15 @@ class Attention(Module):
             self.register_buffer("freqs", rotary_frequencies(dim_head, rotary_theta), persistent=False)
 
     def _norm_rotate(self, q, k, start):
-        eps = self.q_norm.eps if self.q_norm.eps is not None else torch.finfo(torch.float32 if torch.is_autocast_enabled() else q.dtype).eps
-        args = (q, k, self.q_norm.weight, self.k_norm.weight, self.freqs)
+        """One native call, or its plain form; the modules themselves where one is not a plain ``RMSNorm`` of a head (another type, a hook) or
+        they are not alike."""
+        norms = _child(self, "q_norm"), _child(self, "k_norm")
+        if _has_any_global_hook() or any(type(m) is not RMSNorm or m.dim != self.dim_head or _hooked(m) for m in norms) or norms[0].eps != norms[1].eps:
+            q, k = self.q_norm(q), self.k_norm(k)
+            turn = turned(q.shape[1], self.freqs, start)
+            return turn(q.float()).to(q.dtype), turn(k.float()).to(k.dtype)
+        eps = norms[0].eps if norms[0].eps is not None else torch.finfo(torch.float32 if torch.is_autocast_enabled() else q.dtype).eps
+        args = (q, k, _child(norms[0], "weight"), _child(norms[1], "weight"), self.freqs)
         res = _lib.ext().qk_norm_rotary(*args, None, start, eps, False) if q.is_cuda else None
         return res if res is not None else plain_qk_norm_rotary(*args, start, eps)
 
@@ -134,8 +147,7 @@ class TwoSimplicialLM(Module):
         ``nn.Embedding`` (another type, an option, a hook) or the call declines."""
         te, pe = _child(self, "token_emb"), _child(self, "pos_emb")
         plain = x.is_cuda and not _has_any_global_hook() and all(
-            type(m) is nn.Embedding and m.max_norm is None and not m.scale_grad_by_freq and not m.sparse and m.padding_idx is None
-            and not m._forward_hooks and not m._forward_pre_hooks and not m._backward_hooks and not m._backward_pre_hooks and "forward" not in m.__dict__
+            type(m) is nn.Embedding and m.max_norm is None and not m.scale_grad_by_freq and not m.sparse and m.padding_idx is None and not _hooked(m)
             for m in (te, pe))
         if plain:
             res = _lib.ext().embed(x, _child(te, "weight"), _child(pe, "weight"), float(self.embed_scale), start, -1)

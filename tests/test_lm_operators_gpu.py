@@ -223,3 +223,31 @@ def test_threads_at_once():
     for t in threads:
         t.join()
     assert not wrong, wrong[:3]
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_hooks_and_other_modules_of_the_norms(device):
+    torch.manual_seed(8)
+    layer = Attention(dim=64, dim_head=32, heads=4, key_value_heads=2, qk_norm_rotary=True).to(device)
+    x = torch.randn(2, 9, 64, device=device)
+    want = layer(x)
+    seen = []
+    for m in (layer.q_norm, layer.k_norm):
+        m.register_forward_hook(lambda m, a, out: seen.append(m))
+        m.register_full_backward_hook(lambda m, a, g: seen.append(m))
+    got = layer(x)
+    assert seen == [layer.q_norm, layer.k_norm] and (got - want).abs().max() <= 1e-4 * want.abs().max()
+    got.sum().backward()
+    assert len(seen) == 4
+    # a module's result is what is turned
+    layer.k_norm.register_forward_hook(lambda m, a, out: out * 0)
+    assert (layer(x)[:, 0] - want[:, 0]).abs().max() <= 1e-4 * want.abs().max() and not torch.allclose(layer(x)[:, 1:], want[:, 1:], atol=1e-3)
+    other = Attention(dim=64, dim_head=32, heads=4, key_value_heads=2, qk_norm_rotary=True).to(device)
+    other.load_state_dict(layer.state_dict())
+    other.k_norm.eps = 10.0
+    assert not torch.allclose(other(x)[:, 1:], want[:, 1:], atol=1e-3)
+    other.q_norm, other.k_norm = torch.nn.Identity(), torch.nn.Identity()
+    q, k = (f(other.prenorm(x)).view(2, 9, -1, 32) for f in (other.to_q, lambda y: other.to_kv(y).chunk(2, -1)[0]))
+    got = other._norm_rotate(q, k, 5)
+    for a, b in zip(got, (q, k)):
+        assert torch.allclose(a.norm(dim=-1), b.norm(dim=-1), rtol=1e-5) and not torch.allclose(a, b, atol=1e-2)
