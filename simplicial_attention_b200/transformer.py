@@ -129,7 +129,7 @@ class TwoSimplicialLM(Module):
     """Token + learned absolute position embedding, the decoder stack, a linear head
     (train.py:64-135).  ``forward(x, return_loss=True)`` takes ``(b, n + 1)`` token ids and
     returns the next-token cross entropy; with a teacher's largest logits ``(b, n, k)`` and where they stand
-    it returns ``distillation_loss`` against those instead."""
+    it returns ``distillation_loss`` against those instead (CUDA, fp32 or bf16 logits)."""
 
     def __init__(self, *, num_tokens, dim, depth, max_seq_len=1024, dim_head=64, heads=8,
                  two_simplicial_attn_every=4, transformer_kwargs=dict(), embed_scale=1.0):
@@ -159,6 +159,10 @@ class TwoSimplicialLM(Module):
         return tokens + self.pos_emb(torch.arange(start, start + x.shape[-1], device=x.device))
 
     def forward(self, x, return_loss=False, cache=None, return_cache=False, teacher_logits=None, teacher_index=None, temperature=1.0):
+        if (teacher_logits is None) != (teacher_index is None):
+            raise ValueError("a teacher has logits and an index")
+        if teacher_logits is not None and (not return_loss or return_cache):
+            raise ValueError("a teacher is for the loss: return_loss=True, without a cache")
         if return_loss:
             x, target = x[:, :-1], x[:, 1:]
         n = x.shape[-1]
@@ -217,6 +221,8 @@ def training_step(model: Module, optimizer: torch.optim.Optimizer, tokens: torch
     """One step of the reference's loop (train.py:179-194, without gradient accumulation):
     loss, backward, clip to 0.5, Adam step.  Returns the loss tensor (no host sync).  With a teacher's largest logits ``(b, n, k)`` for the
     ``n`` positions before the last token, and where they stand, the loss is ``distillation_loss`` against those."""
+    if (teacher_logits is None) != (teacher_index is None):
+        raise ValueError("a teacher has logits and an index")
     if teacher_logits is None:
         loss = model(tokens, return_loss=True)
         loss.backward()

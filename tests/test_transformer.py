@@ -162,3 +162,19 @@ def test_sampling_draws_from_the_generator(filters):
     a = draw(1)
     assert torch.equal(a, draw(1)) and not torch.equal(a, draw(2))
     assert torch.equal(state, torch.cuda.get_rng_state() if filters else torch.get_rng_state())      # and from nothing else
+
+
+def test_a_teacher_that_no_loss_would_see_is_refused():
+    model = TwoSimplicialLM(num_tokens=20, dim=8, depth=1, dim_head=8, heads=1, transformer_kwargs=dict(key_value_heads=1))
+    tokens, values, index = torch.zeros(2, 6, dtype=torch.long), torch.zeros(2, 5, 3), torch.zeros(2, 5, 3, dtype=torch.long)
+    teacher = dict(teacher_logits=values, teacher_index=index)
+    for kw in (teacher, dict(return_loss=True, return_cache=True, **teacher)):
+        with pytest.raises(ValueError, match="return_loss"):
+            model(tokens, **kw)
+    opt = torch.optim.SGD(model.parameters(), lr=0.1)
+    for half in (dict(teacher_logits=values), dict(teacher_index=index)):
+        with pytest.raises(ValueError, match="index"):
+            model(tokens, return_loss=True, **half)
+        with pytest.raises(ValueError, match="index"):
+            training_step(model, opt, tokens, **half)
+    assert model(tokens).shape == (2, 6, 20) and model(tokens, return_loss=True).shape == ()
