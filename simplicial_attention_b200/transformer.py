@@ -43,6 +43,8 @@ class Attention(Module):
     """Pre-norm causal grouped-query attention (two_simplicial_transformer.py:25-65).  With ``qk_norm_rotary`` (not in the reference)
     queries and keys are normalised per head and turned by position, in one kernel on CUDA."""
 
+    qk_norm_rotary = False      # (of modules pickled without the option)
+
     def __init__(self, dim, dim_head=64, heads=8, key_value_heads=8, qk_norm_rotary=False, rotary_theta=10000.0):
         super().__init__()
         assert divisible_by(heads, key_value_heads)
@@ -130,6 +132,8 @@ class TwoSimplicialLM(Module):
     (train.py:64-135).  ``forward(x, return_loss=True)`` takes ``(b, n + 1)`` token ids and
     returns the next-token cross entropy; with a teacher's largest logits ``(b, n, k)`` and where they stand
     it returns ``distillation_loss`` against those instead (CUDA, fp32 or bf16 logits)."""
+
+    embed_scale = 1.0           # (of modules pickled without the option)
 
     def __init__(self, *, num_tokens, dim, depth, max_seq_len=1024, dim_head=64, heads=8,
                  two_simplicial_attn_every=4, transformer_kwargs=dict(), embed_scale=1.0):

@@ -178,3 +178,13 @@ def test_a_teacher_that_no_loss_would_see_is_refused():
         with pytest.raises(ValueError, match="index"):
             training_step(model, opt, tokens, **half)
     assert model(tokens).shape == (2, 6, 20) and model(tokens, return_loss=True).shape == ()
+
+
+def test_modules_from_before_the_options():
+    """A model unpickled from a time without them has no such attributes."""
+    import pickle
+    model = TwoSimplicialLM(num_tokens=20, dim=8, depth=1, dim_head=8, heads=1, transformer_kwargs=dict(key_value_heads=1))
+    x = torch.arange(12).view(2, 6)
+    want = model(x)
+    del model.__dict__["embed_scale"], model.transformer.layers[0][0].__dict__["qk_norm_rotary"]
+    assert torch.equal(pickle.loads(pickle.dumps(model))(x), want)
