@@ -3,6 +3,8 @@
 Tolerances, with u = 2^-24: a weight 2^x is off by 4 u (ex2) and by 2 u |x| (its exponent's roundings), the sum of a row by at most
 (vocab / 32 + 64) u more, the logarithm and the probabilities by the same.  `slack` below is the sum of these; results are rounded to
 their types."""
+import math
+
 import pytest
 import torch
 
@@ -369,3 +371,26 @@ def test_ruled_out_tokens_of_little_probability(below, vocab, dtype):
     assert total == float("inf") and grad.isfinite().all() and both.isfinite().all()
     keep = [0, 2, 3]
     _check(z.detach()[keep], t[keep], i[keep], 1.0, "none")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("vocab", [301, 2047, 5001, 20001, 40003, 70001])
+def test_every_place_of_a_row_counts_once(vocab, dtype):
+    """A row that one logit dominates, at each place where the reading of a row begins, ends or changes its step, in rows that begin at every distance from a
+    16-byte boundary: left out or taken twice, it would change loss and gradient by a third."""
+    size, threads = torch.finfo(dtype).bits // 8, (32, 128, 256, 512)
+    places = []
+    for r in range(8):                                   # (an odd vocabulary: eight rows have all distances)
+        head = (-r * vocab * size % 16) // size
+        pieces = (vocab - head) // 8
+        ends = {0, head - 1, head, head + 7, head + 8, head + 8 * pieces - 9, head + 8 * pieces - 8, head + 8 * pieces - 1, head + 8 * pieces, vocab - 1, vocab // 2}
+        ends |= {head + 8 * g * v + d for g in threads for v in (1, 2, 4, 8) for d in (-1, 0) if g * v < pieces}
+        ends |= {head + 8 * (pieces - 1 - g * v) + d for g in threads for v in (1, 2, 4, 8) for d in (7, 8) if g * v < pieces}
+        places.append(sorted(p for p in ends if 0 <= p < vocab))
+    count = max(map(len, places))
+    where = torch.tensor([places[r % 8][(r // 8) % len(places[r % 8])] for r in range(8 * count)], device="cuda")
+    z, t, i = _inputs(8 * count, vocab, 4, dtype, spread=0.5)
+    z.scatter_(1, where[:, None], torch.full_like(z[:, :1], math.log(vocab) + 1))
+    i[::2, 0] = where[::2]
+    i[:, 1:] = torch.where(i[:, 1:] == i[:, :1], torch.full_like(i[:, 1:], -1), i[:, 1:])
+    _check(z, t, i)
