@@ -122,6 +122,7 @@ struct BwdParams {
     int64_t rows, vocab, padding, start, position_rows;
     int n, dim, passes, bits;   // sort: passes of `bits` bits; the sorted keys are in key[passes & 1]
     int tiles;                  // pieces of a row
+    int zeroing;                // CTAs that write zeros
     float scale;
 };
 
@@ -168,12 +169,15 @@ __device__ __forceinline__ void warp_zeros(char *p, int64_t bytes) {
     if (lane < (bytes & 15)) p[(bytes & ~(int64_t)15) + lane] = 0;
 }
 
-// Zeros of the tokens that are not there, of the words [first, last) of 32 tokens each: a CTA, `bits` of WORDS words
+// Zeros of the tokens of [first, last) that are not there: a CTA, `bits` of WORDS words, which say of 32 tokens each that there is nothing to do
 __device__ __forceinline__ void zero_absent(const BwdParams &P, int64_t first, int64_t last, uint32_t *bits, int64_t row_bytes) {
-    for (int64_t w0 = first; w0 < last; w0 += WORDS) {
-        const int words = (int)min((int64_t)WORDS, last - w0);
+    for (int64_t w0 = first / 32; w0 * 32 < last; w0 += WORDS) {
+        const int words = (int)min((int64_t)WORDS, (last + 31) / 32 - w0);
         __syncthreads();
-        for (int x = threadIdx.x; x < words; x += SORT_THREADS) bits[x] = 0u;
+        for (int x = threadIdx.x; x < words; x += SORT_THREADS) {
+            const int64_t t0 = (w0 + x) * 32;
+            bits[x] = (t0 < first ? (1u << (first - t0)) - 1u : 0u) | (t0 + 32 > last ? ~0u << (last - t0) : 0u);
+        }
         __syncthreads();
         constexpr int U = 4;
         for (int64_t x0 = threadIdx.x; x0 < P.rows; x0 += U * SORT_THREADS) {
@@ -192,10 +196,8 @@ __device__ __forceinline__ void zero_absent(const BwdParams &P, int64_t first, i
         while (group < 32 && 2 * group * row_bytes <= 2048) group *= 2;
         for (int x = threadIdx.x >> 5; x < words * (32 / group); x += SORT_WARPS) {
             const int64_t t0 = w0 * 32 + (int64_t)x * group;
-            if (t0 >= P.vocab) break;
             uint32_t absent = ~bits[x * group / 32] >> (x * group % 32);
-            const int most = (int)min((int64_t)group, P.vocab - t0);
-            if (most < 32) absent &= (1u << most) - 1u;
+            if (group < 32) absent &= (1u << group) - 1u;
             while (absent) {
                 const int from = __ffs(absent) - 1, behind = ~(absent >> from) ? __ffs(~(absent >> from)) - 1 : 32, count = min(behind, 32 - from);
                 warp_zeros(reinterpret_cast<char *>(P.dweight) + (t0 + from) * row_bytes, count * row_bytes);
@@ -216,8 +218,9 @@ __global__ void __launch_bounds__(SORT_THREADS, 2) sort_kernel(const __grid_cons
     if ((int)blockIdx.x >= sorting) {
         const int64_t cta = blockIdx.x - sorting, others = gridDim.x - sorting;
         if (P.dweight) {
-            const int64_t words = (P.vocab + 31) / 32, each = (words + others - 1) / others;
-            zero_absent(P, min(words, cta * each), min(words, (cta + 1) * each), smem, (int64_t)P.dim * sizeof(T));
+            int64_t each = (P.vocab + P.zeroing - 1) / P.zeroing;
+            if (each > SORT_WARPS && each < 4 * SORT_WARPS) each = (each + SORT_WARPS - 1) / SORT_WARPS * SORT_WARPS;
+            if (cta < P.zeroing) zero_absent(P, min(P.vocab, cta * each), min(P.vocab, (cta + 1) * each), smem, (int64_t)P.dim * sizeof(T));
         }
         const int64_t units = P.position_rows * P.tiles;
         for (int64_t u = cta * SORT_WARPS + warp; P.dpositions && u < units; u += others * SORT_WARPS) add_positions<T, V>(P, u);
@@ -451,6 +454,18 @@ inline int sort_ctas(int64_t rows) {
     int c = 1;
     while (c < SORT_CTAS && rows > (int64_t)c * SORT_THREADS) c *= 2;
     return c;
+}
+// CTAs beside the sort: two an SM, as many as clusters of that many CTAs find room for
+inline int others_at_most(int cluster, int sms) { return cluster == SORT_CTAS ? 216 : 2 * sms - 2 * cluster; }
+// CTAs that write zeros: one for 512 tokens; more where rows that no token can name weigh more than 128 KB each of them.  Each looks through all
+// tokens: where those are few, CTAs go on coming, 512 KB each, which the SMs take as they get through (32 tokens, 128000 x 4096 fp32 of a
+// table: 412 us with 216 CTAs, 352 with 286, 310 with 4000; one token, 8192 x 4096: 142 with 16, 29 with 256; 131072 tokens, 50257 x 768: 189 with 99,
+// 199 with 216).
+inline int zero_ctas(int64_t rows, int64_t vocab, int64_t row_bytes, int most) {
+    const int64_t few = (vocab + 511) / 512, sure = vocab > rows ? (vocab - rows) * row_bytes : 0, heavy = sure / (128 * 1024);
+    int64_t c = few > heavy ? few : heavy;
+    if (c > most) c = rows <= 4 * SORT_THREADS && sure / (512 * 1024) > most ? sure / (512 * 1024) : most;
+    return (int)(c < 65536 ? c : 65536);
 }
 inline size_t sort_smem(int bits) {
     const size_t sort = ((size_t)SORT_WARPS + 1) * ((size_t)1 << bits) * 4 + SORT_WARPS * 4;

@@ -132,11 +132,11 @@ template <typename T, int V> int embed_bwd_run(sa2::embed::BwdParams P, cudaStre
     using namespace sa2::embed;
     P.tiles = embed_tiles(P.dim, V == 8);
     const int sorting = P.dweight ? sort_ctas(P.rows) : 0, cluster = sorting ? sorting : 1;
-    // the others: a warp for 256 channels of a row of dP, and for 32 tokens' zeros; of two CTAs an SM, as many as clusters of eight
-    // find room beside the sort
-    const int64_t zeros = P.dweight ? (P.vocab + 31) / 32 : 0, adding = P.dpositions ? P.position_rows * P.tiles : 0;
-    int64_t others = ((zeros > adding ? zeros : adding) + SORT_WARPS - 1) / SORT_WARPS;
-    if (others > 216) others = 216;
+    // the others: a warp for 256 channels of a row of dP
+    const int64_t most = others_at_most(cluster, SM_COUNT), adding = P.dpositions ? (P.position_rows * P.tiles + SORT_WARPS - 1) / SORT_WARPS : 0;
+    P.zeroing = P.dweight ? zero_ctas(P.rows, P.vocab, P.dim * (int64_t)sizeof(T), (int)most) : 0;
+    int64_t others = adding < most ? adding : most;
+    if (others < P.zeroing) others = P.zeroing;
     others = (others + cluster - 1) / cluster * cluster;
     if (int e = launch_clusters(sort_kernel<T, V>, sorting + others, SORT_THREADS, sort_smem(P.bits), cluster, st, P, sorting)) return e;
     if (!P.dweight) return SA2_OK;

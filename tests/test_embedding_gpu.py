@@ -220,3 +220,64 @@ def test_positions_behind_the_table_are_refused():
         with pytest.raises(ValueError, match="positions"):
             sa.token_embedding(tokens, weight, pos, start=start)
     assert sa.token_embedding(tokens, weight, pos, start=10).shape == (2, 30, 16)
+
+
+def _c_backward(tokens, vocab, dim, dtype, positions=0):
+    """The C entry's gradients in memory that held NaN, and a call that repeats it."""
+    import ctypes as C
+
+    from test_operator_refusals import EmbedArgs
+    lib = _lib.lib()
+    lib.sa2_embed_workspace_bytes.restype = C.c_size_t
+    dout = torch.randn(*tokens.shape, dim, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda").to(dtype)
+    dweight = torch.full((vocab, dim), float("nan"), device="cuda", dtype=dtype)
+    dpositions = torch.full((positions, dim), float("nan"), device="cuda", dtype=dtype)
+    ws = torch.empty(lib.sa2_embed_workspace_bytes(C.c_int64(tokens.numel()), C.c_int32(dim)), dtype=torch.uint8, device="cuda")
+    a = EmbedArgs(tokens=tokens.data_ptr(), dout=dout.data_ptr(), dweight=dweight.data_ptr(), dpositions=dpositions.data_ptr() if positions else None, workspace=ws.data_ptr(),
+                  workspace_bytes=ws.numel(), rows=tokens.numel(), vocab=vocab, n=tokens.shape[-1], dim=dim, position_rows=positions, tokens64=1, padding=-1, scale=1.0,
+                  dtype=_lib.SA2_F32 if dtype == torch.float32 else _lib.SA2_BF16, stream=torch.cuda.current_stream().cuda_stream)
+
+    def call():
+        assert lib.sa2_embed_bwd(C.byref(a)) == 0
+
+    call()
+    return call, dout, dweight, dpositions, ws
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("rows", [1, 33, 700, 3000])
+@pytest.mark.parametrize("vocab, dim", [(1, 4096), (2, 70000), (65, 8200), (333, 4096), (5003, 4096), (8192, 1000), (8191, 2049), (40009, 1031), (300007, 65)], ids=str)
+def test_zeros_of_tokens_that_are_not_there(vocab, dim, rows, dtype):
+    """Wide and narrow tables around the sizes at which more CTAs share the zeros: each row of the gradient is written, by one of them."""
+    gen = torch.Generator(device="cuda").manual_seed(rows)
+    tokens = torch.randint(vocab, (1, rows), generator=gen, device="cuda")
+    tokens[0, 0] = vocab - 1
+    for positions in (0, rows + 3):
+        _, dout, dweight, dpositions, _ = _c_backward(tokens, vocab, dim, dtype, positions)
+        count = torch.bincount(tokens[0], minlength=vocab)
+        assert (dweight[count == 0] == 0).all()
+        once = (count == 1).nonzero()[:, 0]
+        place = torch.empty(vocab, dtype=torch.long, device="cuda").scatter_(0, tokens[0], torch.arange(rows, device="cuda"))
+        assert torch.equal(dweight[once], dout[0, place[once]]) and not dweight.isnan().any()
+        if positions:
+            assert torch.equal(dpositions[:rows], dout[0]) and (dpositions[rows:] == 0).all()
+
+
+@pytest.mark.parametrize("vocab", [8192, 128000])
+def test_few_tokens_of_a_wide_table_cost_little_more_than_its_zeros(vocab):
+    """A step with a handful of tokens is bound by the zeros of the dense gradient, whatever the table's shape: with CTAs counted by the vocabulary alone,
+    one token of 8192 took seven times the time of a fill."""
+    call, _, dweight, _, ws = _c_backward(torch.tensor([[5]], device="cuda"), vocab, 4096, torch.float32)
+
+    def best(f):
+        times = []
+        for _ in range(10):
+            start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            start.record()
+            f()
+            end.record()
+            end.synchronize()
+            times.append(start.elapsed_time(end))
+        return min(times)
+
+    assert best(call) <= 3 * best(dweight.zero_)
