@@ -314,7 +314,7 @@ int sa2_distill_bwd(const sa2_distill_args *a) {
 int sa2_distill_both(const sa2_distill_args *a) {
     Range range("sa2_distill_both");
     if (int e = distill_check(a, true, true)) return e;
-    if (a->gout || !a->total) return SA2_ERR_INVALID;
+    if (a->gout || !a->total || a->grad_scale * 0.f != 0.f) return SA2_ERR_INVALID;
     return a->dtype == SA2_BF16 ? distill_fwd<__nv_bfloat16>(a, true) : distill_fwd<float>(a, true);
 }
 

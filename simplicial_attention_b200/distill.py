@@ -5,8 +5,6 @@ The reference trains on next tokens alone (train.py:129-135).  The CUDA kernels 
 """
 from __future__ import annotations
 
-import math
-
 import torch
 from torch import Tensor
 
@@ -55,7 +53,7 @@ def distillation_loss_and_grad(logits: Tensor, teacher_logits: Tensor, teacher_i
     that goes backward at once: ``logits.backward(grad)``.  It reads the logits from memory once where autograd's two calls read them twice.
     ``grad_scale`` is what the loss would be multiplied with before its backward (a loss scale, one over accumulated steps)."""
     _check(temperature, reduction, ("mean", "sum"))
-    if not math.isfinite(grad_scale):
-        raise ValueError(f"grad_scale must be finite, not {grad_scale}")
+    if not abs(grad_scale) <= torch.finfo(torch.float32).max:           # fp32 in the kernels
+        raise ValueError(f"grad_scale must be finite in fp32, not {grad_scale}")
     res = _lib.ext().distill_both(logits, teacher_logits, teacher_index, float(temperature), _REDUCTIONS[reduction], float(grad_scale))
     return res if res is not None else _refuse(logits, teacher_logits, teacher_index, temperature, reduction, _REDUCTIONS)

@@ -237,3 +237,13 @@ def test_widths_next_to_the_largest_int():
         assert lib.sa2_embed_fwd(C.byref(a)) == 2 and lib.sa2_embed_bwd(C.byref(a)) == 2
     with pytest.raises(ValueError, match="2\\^30"):
         sa.token_embedding(_cuda(2, 3, dtype=torch.long), _cuda(1, 2 ** 30 + 8))
+
+
+def test_gradient_scales_beyond_fp32():
+    z, t, i = _cuda(4, 50), _cuda(4, 3), _cuda(4, 3, dtype=torch.long)
+    for scale in (1e39, -1e39, math.inf):
+        with pytest.raises(ValueError, match="grad_scale"):
+            sa.distillation_loss_and_grad(z, t, i, grad_scale=scale)
+    good = dict(logits=A, teacher=A, index=A, total=A, dlogits=A, workspace=A, workspace_bytes=1 << 20, rows=3, vocab=9, k=2, temperature=1.0)
+    for scale in (math.inf, -math.inf, math.nan):
+        assert _lib.lib().sa2_distill_both(C.byref(DistillArgs(**{**good, "grad_scale": scale}))) == 1
