@@ -288,7 +288,7 @@ __device__ __forceinline__ double term(float prob, float logit, float best, doub
     const double x = ((double)logit - (double)best) * inv_t;
     return x == -CUDART_INF ? x : (double)prob * x;
 }
-__device__ __forceinline__ float row_loss(double self, float s, double terms, float t) { return (float)((self + log((double)s) - terms) * (double)t * (double)t); }
+__device__ __forceinline__ float row_loss(double self, double log_s, double terms, float t) { return (float)((self + log_s - terms) * (double)t * (double)t); }
 
 // Running maximum and sum of exponentials of what a thread has seen
 template <typename T> struct Running {
@@ -395,7 +395,7 @@ __global__ void __launch_bounds__(G == 32 ? 256 : G, G == 32 ? 4 : 1536 / G) fwd
     }
     const float2 all = joined<G, T>(run.result(), of_warp, f);
     const float best = all.x == -CUDART_INF_F ? 0.f : all.x, s = all.y;
-    const double inv_t = 1. / (double)P.t;
+    const double log_s = log((double)s), inv_t = 1. / (double)P.t;       // (the logarithm here: behind the sum over warps it made registers spill)
     double terms = 0.;
     for (int k = Group<G>::rank(); k < P.k; k += G) {
         const int i = P.place[r * P.k + k];
@@ -405,7 +405,7 @@ __global__ void __launch_bounds__(G == 32 ? 256 : G, G == 32 ? 4 : 1536 / G) fwd
     if (Group<G>::rank() == 0) {
         P.stats[2 * r] = best;
         P.stats[2 * r + 1] = s;
-        P.row_loss[r] = row_loss(P.self[r], s, terms, P.t);
+        P.row_loss[r] = row_loss(P.self[r], log_s, terms, P.t);
     }
 }
 
@@ -478,7 +478,7 @@ __global__ void __launch_bounds__(G, 1024 / G) both_kernel(const __grid_constant
     if (threadIdx.x == 0) {
         double terms = 0.;
         for (int w = 0; there && w < G / 32 && w * 32 < P.k; ++w) terms += terms_of[w];
-        P.row_loss[r] = there ? row_loss(P.self[r], s, terms, P.t) : 0.f;
+        P.row_loss[r] = there ? row_loss(P.self[r], log((double)s), terms, P.t) : 0.f;
     }
 }
 
