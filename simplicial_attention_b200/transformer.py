@@ -131,7 +131,8 @@ class TwoSimplicialLM(Module):
     """Token + learned absolute position embedding, the decoder stack, a linear head
     (train.py:64-135).  ``forward(x, return_loss=True)`` takes ``(b, n + 1)`` token ids and
     returns the next-token cross entropy; with a teacher's largest logits ``(b, n, k)`` and where they stand
-    it returns ``distillation_loss`` against those instead (CUDA, fp32 or bf16 logits)."""
+    it returns ``distillation_loss`` against those instead (CUDA, fp32 or bf16 logits).  On CUDA a token outside of the table has NaN for an
+    embedding, and ``sample_tokens`` answers -1 for logits of NaN; on the CPU it is torch's ``IndexError``."""
 
     embed_scale = 1.0           # (of modules pickled without the option)
 
@@ -150,6 +151,8 @@ class TwoSimplicialLM(Module):
         """Token and position embeddings of rows ``start`` on: one native call, or the two modules where one of them is not a plain
         ``nn.Embedding`` (another type, an option, a hook) or the call declines."""
         te, pe = _child(self, "token_emb"), _child(self, "pos_emb")
+        if type(pe) is nn.Embedding and not _hooked(pe) and start + x.shape[-1] > pe.num_embeddings:
+            raise IndexError(f"{start + x.shape[-1]} rows are more than the table's {pe.num_embeddings} positions")
         plain = x.is_cuda and not _has_any_global_hook() and all(
             type(m) is nn.Embedding and m.max_norm is None and not m.scale_grad_by_freq and not m.sparse and m.padding_idx is None and not _hooked(m)
             for m in (te, pe))

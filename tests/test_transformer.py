@@ -188,3 +188,15 @@ def test_modules_from_before_the_options():
     want = model(x)
     del model.__dict__["embed_scale"], model.transformer.layers[0][0].__dict__["qk_norm_rotary"]
     assert torch.equal(pickle.loads(pickle.dumps(model))(x), want)
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_positions_behind_the_table_are_refused(device):
+    """On the host: on a GPU torch's lookup of such a position ends the context."""
+    model = TwoSimplicialLM(num_tokens=20, dim=8, depth=1, dim_head=8, heads=1, max_seq_len=6, transformer_kwargs=dict(key_value_heads=1)).to(device)
+    x = torch.zeros(2, 6, dtype=torch.long, device=device)
+    with pytest.raises(IndexError, match="6 positions"):
+        model(torch.cat((x, x), dim=1))
+    with pytest.raises(IndexError, match="6 positions"):
+        model.sample(x, 8)
+    assert model(x).shape == (2, 6, 20) and model.sample(x[:, :3], 6).shape == (2, 3)
