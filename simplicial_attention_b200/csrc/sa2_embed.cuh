@@ -12,7 +12,8 @@
 // chain of latencies that a few SMs do as fast as all of them.  (2) A warp adds a stretch of sorted places for 256 channels, rows of
 // dout read whole; a token whose places all lie in the stretch is finished there, one that began or goes on elsewhere leaves a partial row.
 // (3) Partial rows of a token are added in order.  16384 tokens, 50001 of 2048 bf16 channels: 40, 27 and 9 us (zeros of the whole table beside
-// the sort, written twice where tokens are: 40 and 49); 16384 of 256 tokens, 512 fp32 channels: 13, 8 and 4.  Sums are fp32 and have one order, whatever the run: no floating-point atomics.
+// the sort, written twice where tokens are: 40 and 49); 16384 of 256 tokens, 512 fp32 channels: 13 (10 without the positions' sums), 8 and 4.  Sums are
+// fp32 and have one order, whatever the run: no floating-point atomics.
 #pragma once
 #include "sa2_common.cuh"
 #include "sa2_vec8.cuh"
@@ -449,7 +450,7 @@ inline void sort_plan(int64_t vocab, int &passes, int &bits) {
     passes = (all + 8) / 9;
     bits = (all + passes - 1) / passes;
 }
-// CTAs of the sort: 1024 places each, a power of two
+// CTAs of the sort: a power of two, up to 512 places each until there are eight
 inline int sort_ctas(int64_t rows) {
     int c = 1;
     while (c < SORT_CTAS && rows > (int64_t)c * SORT_THREADS) c *= 2;
