@@ -18,7 +18,7 @@
 // adds up the masses before each.  Otherwise what is in the bracket is cut again first, on the bits of the logits mapped to integers in
 // their order, with exact masses, 512 stretches at a time.  (4) Warps add the kept masses, and the one that has the drawn mass walks its list.
 // Bound: reading the logits once, of which few calls come near: one row of 256 12 us and 64 rows of 32000 21 us (chains of waits), 256 rows of
-// 128000 fp32 logits 120 to 175 us and 410 to 470 where the cut lies among many (a floor of 20: the second reading from L2 and HBM, the masses'
+// 128000 fp32 logits 110 to 175 us and 410 to 470 where the cut lies among many (a floor of 20: the second reading from L2 and HBM, the masses'
 // 64-bit arithmetic, and the second row of an SM's two CTAs where 256 rows are no multiple of the places); 16384 rows of 256 logits 182 us (a floor
 // of 3: a CTA, its tables and about ten waits for so short a row).
 #pragma once
